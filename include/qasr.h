@@ -350,6 +350,109 @@ QASR_API int qasr_op_conv3x3_gelu(const void* in, int32_t n_chunks, int32_t Hi, 
 QASR_API int qasr_op_fbank(const float* pcm, int64_t n, float* feats /*[T][80]*/, void* stream);
 QASR_API int qasr_stream_sync(void* stream);
 
+/* -------------------------------------------------------------------------------------------- paged K/V cache */
+/* A K/V cache in pages, for servers whose sessions grow to lengths nobody knows beforehand, and the operators that meet
+   in one step over it: rotary positions, appending, attention.  They take device pointers and a hipStream_t like every
+   qasr_op_*, allocate nothing, do not synchronise and can be captured into a graph.  The stream (NULL = the null stream)
+   has to belong to the calling thread's current device (QASR_E_INVALID otherwise) and the pointers to be reachable from
+   it.  Descriptions (qasr_kv_cache, qasr_rope, qasr_paged_attn) are read during the call only.  What a kernel finds on
+   the device — positions, page ids, lengths — is checked there: see each operator for what an entry out of range does;
+   none is ever followed out of a buffer.
+
+   Pages: a pool [page][KV head] of blocks of page_size tokens, K and V each with its own pool of qasr_kv_pool_bytes.
+     QASR_T_F16 / QASR_T_BF16   block = [token][head_dim]
+     QASR_T_MXFP4               4-bit floats (e2m1: 0 .5 1 1.5 2 3 4 6 and their negatives, code 8 + c = -c) times one power
+       of two 2^E per 32 dims, as OCP MXFP4: 17/32 byte an element.  E is the smallest exponent with max |x| <= 6 * 2^E,
+       kept in [-23, 13] so that every value is exact in f16 and bf16 (larger inputs saturate at 49152); a code is the
+       nearest value, ties to the even code.  A block of 32 that holds an infinity or NaN reads back as NaN.
+       block = page_size * head_dim / 2 bytes of codes, then page_size * head_dim / 32 scale bytes E + 127 (255 = NaN):
+         K codes   per token, dims in the order ((d % 32) / 8, d / 32, d % 8), the even dim in a byte's low half
+         K scales  [token][head_dim / 32]
+         V codes   per 16 tokens in the order ((t % 16) / 4, d / (head_dim / 16), t % 4, d % (head_dim / 16))
+         V scales  per 16 tokens [head_dim / 32][16]
+   page_table[seq][i] is the page of the sequence's tokens [i * page_size, (i + 1) * page_size); sequences may share pages
+   that nobody appends to. */
+enum { QASR_T_F32 = 0, QASR_T_F16 = 1, QASR_T_BF16 = 2, QASR_T_MXFP4 = 3 };
+typedef struct {
+    void* k;                   /* pools, 16-byte aligned */
+    void* v;
+    const int32_t* page_table; /* device [n_seq][max_pages] */
+    int32_t n_seq, max_pages;
+    int32_t n_pages;           /* pages in a pool; an id outside [0, n_pages) stands for no page */
+    int32_t page_size;         /* a power of two, 16 .. 1024 */
+    int32_t n_kv_heads;        /* 1 .. 1024 */
+    int32_t head_dim;          /* 64, 128 or 256 */
+    int32_t type;              /* QASR_T_F16, QASR_T_BF16 or QASR_T_MXFP4 */
+} qasr_kv_cache;
+QASR_API int qasr_kv_pool_bytes(const qasr_kv_cache* c, size_t* bytes);
+
+/* What happens to a head before it is used: y = x, or x / sqrt(mean(x^2) + eps) * norm_w over the head where norm_w is
+   given; then for the pairs (a, b) of its first rot_dim dims — dims i and i + rot_dim / 2, or 2i and 2i + 1 (interleaved)
+   — a' = a cos - b sin, b' = b cos + a sin with row `position` of the table.  The other dims pass. */
+typedef struct {
+    const float* cs;       /* device [n_pos][rot_dim / 2][2] cos, sin, 8-byte aligned; NULL = no rotation */
+    int32_t n_pos;         /* rows of cs */
+    int32_t rot_dim;       /* even, <= head_dim */
+    int32_t interleaved;
+    const float* norm_w;   /* device [head_dim] or NULL */
+    float eps;
+} qasr_rope;
+enum { QASR_ROPE_PLAIN = 0, QASR_ROPE_LINEAR = 1, QASR_ROPE_NTK = 2, QASR_ROPE_YARN = 3 };
+typedef struct {
+    int32_t rot_dim;       /* even, >= 2 (NTK: >= 4) */
+    int32_t kind;
+    double theta;          /* > 0 (YaRN: > 1): frequency i is theta^(-2i / rot_dim) */
+    double factor;         /* >= 1; unused by PLAIN.  LINEAR: every frequency / factor.  NTK: theta * factor^(rot / (rot - 2)) */
+    double orig_ctx;       /* YARN: the trained context; */
+    double beta_fast, beta_slow;   /* frequencies that turn more than beta_fast times over it stay, fewer than beta_slow
+                                      are divided by factor, between them a ramp; cos and sin times 0.1 ln(factor) + 1 */
+} qasr_rope_scaling;
+/* cos / sin of the positions first .. first + n_pos - 1 from 64-bit angles into cs (device [n_pos][rot_dim / 2][2]) */
+QASR_API int qasr_op_rope_table_scaled(const qasr_rope_scaling* r, int64_t first, int32_t n_pos, float* cs, void* stream);
+/* y[row][head] = the head as qasr_rope says, at position pos[row] (pos may be NULL without a rotation).  x_type and
+   y_type: QASR_T_F32 / F16 / BF16; rows are ldx / ldy elements apart (>= heads * head_dim, any alignment), head_dim even, <= 1024.
+   A row whose position is not in [0, n_pos) is padding: its y stays as it was.  y may be x (same type and stride).
+   Arithmetic in 32 bits, one rounding at the end. */
+QASR_API int qasr_op_rope(const void* x, int32_t x_type, int64_t ldx, const int32_t* pos, int32_t rows, int32_t heads,
+                          int32_t head_dim, const qasr_rope* rope, void* y, int32_t y_type, int64_t ldy, void* stream);
+/* Row r's K heads (k + r * ldk, as `rope` says, NULL = as they are) and V heads (as they are) to position pos[r] of
+   sequence seq[r].  x_type as above.  Rows with seq outside [0, n_seq), pos outside [0, max_pages * page_size) (or the
+   table's rows, where there is a rotation) or no page there are padding and write nothing.  Where two rows name the same
+   place, what it holds afterwards is unspecified.  Into 16-bit pages in 32-bit arithmetic; into MXFP4 pages the rotation is computed in 64 bits and
+   rounded to f32 before the codes are chosen. */
+QASR_API int qasr_op_kv_append(const qasr_kv_cache* c, const void* k, const void* v, int32_t x_type, int64_t ldk,
+                               int64_t ldv, const int32_t* seq, const int32_t* pos, int32_t rows, const qasr_rope* rope,
+                               void* stream);
+/* The inverse, without the rotation: the values held for (seq[r], pos[r]) into rows of k and v (either may be NULL), y_type
+   QASR_T_F32 / F16 / BF16.  Rows that append would skip are left as they were. */
+QASR_API int qasr_op_kv_gather(const qasr_kv_cache* c, const int32_t* seq, const int32_t* pos, int32_t rows, void* k,
+                               void* v, int32_t y_type, int64_t ldk, int64_t ldv, void* stream);
+
+/* Attention of packed query rows over the cache.  Sequence s owns rows [q_start[s], q_start[s + 1]) of q and o, n in all,
+   and kv_len[s] keys; its row i sits at position p = kv_len[s] - n + i and sees all of them, or those at positions <= p
+   (causal), of these the positions > p - window (window > 0).  o = softmax(scale * q . k) v per head (query head h reads KV head
+   h / (n_heads / n_kv_heads)); a row that sees no key gets zeros.  One token per sequence (decode), several (verify
+   passes), whole prompts and, without causal, another sequence's states (cross attention) are all this one call.
+   Scores, softmax and sums in 32 bits; the weights are rounded to q's type for the product with V.
+   What lies in a cache outside a sequence's keys is never used, whatever it holds; keys on a page id outside the
+   pool are left out.  kv_len is cut to max_pages * page_size (below 0: 0), q_start's rows to [0, rows); rows that
+   belong to no sequence are left as they were. */
+typedef struct {
+    int32_t n_heads;       /* a multiple of n_kv_heads */
+    int32_t q_type;        /* QASR_T_F16 or QASR_T_BF16; the cache's own type where that is a 16-bit one */
+    int32_t o_type;        /* q_type or QASR_T_F32 */
+    int32_t causal, window;
+    float scale;
+    int32_t max_q, max_kv; /* the most rows / keys that a sequence is expected to have: they choose how the work is split
+                              (more are computed all the same, more slowly) */
+} qasr_paged_attn;
+/* Bytes of scratch for calls with these descriptions; zero it once, every call leaves it ready for the next.  A scratch
+   serves one call at a time: calls (or graphs) that may overlap need one each. */
+QASR_API int qasr_paged_attention_workspace(const qasr_kv_cache* c, const qasr_paged_attn* a, size_t* bytes);
+QASR_API int qasr_op_paged_attention(const qasr_kv_cache* c, const qasr_paged_attn* a, const void* q, int64_t ldq,
+                                     const int32_t* q_start /* [n_seq + 1] */, const int32_t* kv_len /* [n_seq] */,
+                                     int32_t rows, void* o, int64_t ldo, void* ws, size_t ws_bytes, void* stream);
+
 /* Deterministic mode (process-wide, DEFAULT ON; QASR_ATOMICS=1 in the environment starts the process with it off):
    GEMMs never add split-K partial sums with float atomics (whose landing order varies run to run, a last-ulp
    difference that can flip a near-tie) — splits go through the ordered fix-up or do not happen — so every run of

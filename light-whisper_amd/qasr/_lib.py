@@ -17,6 +17,8 @@ VAD_ASSET = os.path.join(REPO_ROOT, "assets", "fireredvad_dfsmn.qvad")
 
 QASR_OK = 0
 EPI_STORE, EPI_RESID, EPI_GELU = 0, 1, 2
+T_F32, T_F16, T_BF16, T_MXFP4 = 0, 1, 2, 3            # element types of the paged K/V cache operators
+ROPE_PLAIN, ROPE_LINEAR, ROPE_NTK, ROPE_YARN = 0, 1, 2, 3
 
 
 class QasrError(RuntimeError):
@@ -56,6 +58,26 @@ class VadOptions(C.Structure):
 
 class Segment(C.Structure):
     _fields_ = [("start", C.c_int64), ("end", C.c_int64)]
+
+
+class KvCache(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("page_table", C.c_void_p)] + [(n, C.c_int32) for n in (
+        "n_seq", "max_pages", "n_pages", "page_size", "n_kv_heads", "head_dim", "type")]
+
+
+class Rope(C.Structure):
+    _fields_ = [("cs", C.c_void_p), ("n_pos", C.c_int32), ("rot_dim", C.c_int32), ("interleaved", C.c_int32),
+                ("norm_w", C.c_void_p), ("eps", C.c_float)]
+
+
+class RopeScaling(C.Structure):
+    _fields_ = [("rot_dim", C.c_int32), ("kind", C.c_int32)] + [(n, C.c_double) for n in (
+        "theta", "factor", "orig_ctx", "beta_fast", "beta_slow")]
+
+
+class PagedAttn(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("n_heads", "q_type", "o_type", "causal", "window")] + [
+        ("scale", C.c_float), ("max_q", C.c_int32), ("max_kv", C.c_int32)]
 
 
 # every exported symbol with (restype, argtypes); the not-gpu test checks each one is exported
@@ -163,6 +185,14 @@ SIGNATURES = {
     "qasr_op_conv3x3_gelu": (C.c_int, [P, I32, I32, I32, P, P, I32, P, I32, P]),
     "qasr_op_fbank": (C.c_int, [P, I64, P, P]),
     "qasr_stream_sync": (C.c_int, [P]),
+    "qasr_kv_pool_bytes": (C.c_int, [C.POINTER(KvCache), C.POINTER(SZ)]),
+    "qasr_op_rope_table_scaled": (C.c_int, [C.POINTER(RopeScaling), I64, I32, P, P]),
+    "qasr_op_rope": (C.c_int, [P, I32, I64, P, I32, I32, I32, C.POINTER(Rope), P, I32, I64, P]),
+    "qasr_op_kv_append": (C.c_int, [C.POINTER(KvCache), P, P, I32, I64, I64, P, P, I32, C.POINTER(Rope), P]),
+    "qasr_op_kv_gather": (C.c_int, [C.POINTER(KvCache), P, P, I32, P, P, I32, I64, I64, P]),
+    "qasr_paged_attention_workspace": (C.c_int, [C.POINTER(KvCache), C.POINTER(PagedAttn), C.POINTER(SZ)]),
+    "qasr_op_paged_attention": (C.c_int, [C.POINTER(KvCache), C.POINTER(PagedAttn), P, I64, P, P, I32, P, I64, P, SZ,
+                                          P]),
     "qasr_prof_enable": (C.c_int, [C.c_int]),
     "qasr_set_deterministic": (C.c_int, [I32]),
     "qasr_get_deterministic": (C.c_int, [P]),
