@@ -377,7 +377,7 @@ typedef struct {
     void* k;                   /* pools, 16-byte aligned */
     void* v;
     const int32_t* page_table; /* device [n_seq][max_pages] */
-    int32_t n_seq, max_pages;
+    int32_t n_seq, max_pages;  /* max_pages * page_size <= 2^30 */
     int32_t n_pages;           /* pages in a pool; an id outside [0, n_pages) stands for no page */
     int32_t page_size;         /* a power of two, 16 .. 1024 */
     int32_t n_kv_heads;        /* 1 .. 1024 */

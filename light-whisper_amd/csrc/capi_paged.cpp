@@ -33,8 +33,8 @@ KvPages pages_of(const qasr_kv_cache* c, bool pools) {
     QASR_CHECK(c->page_size >= 16 && c->page_size <= 1024 && (c->page_size & (c->page_size - 1)) == 0, QASR_E_INVALID,
                "kv cache: page_size must be a power of two from 16 to 1024");
     QASR_CHECK(c->n_pages >= 0 && c->n_seq >= 0 && c->max_pages >= 0, QASR_E_INVALID, "kv cache: negative count");
-    QASR_CHECK((int64_t)c->max_pages * c->page_size <= INT_MAX, QASR_E_INVALID,
-               "kv cache: max_pages * page_size must stay below 2^31 positions");
+    QASR_CHECK((int64_t)c->max_pages * c->page_size <= 1 << 30, QASR_E_INVALID,
+               "kv cache: max_pages * page_size must be at most 2^30 positions");
     if (pools) {
         QASR_CHECK(c->n_pages == 0 || (c->k && c->v), QASR_E_INVALID, "kv cache: NULL pool");
         QASR_CHECK(aligned(c->k, 16) && aligned(c->v, 16), QASR_E_INVALID, "kv cache: pools must be 16-byte aligned");

@@ -85,9 +85,9 @@ class Pool:
 
 def attend(q, k, v, q_start, kv_len, table, scale, causal, window, out):
     """q [rows][nh][hd]; k, v [pages][nkv][page][hd] values (f64) -> out (filled for rows of a sequence), and the
-    weighted mean of |v| that the tolerances go by."""
+    weighted mean and the plain sum of |v| that the tolerances go by."""
     nh, nkv, page, n_pages = q.shape[1], k.shape[1], k.shape[2], k.shape[0]
-    mag = np.zeros_like(out)
+    mag, total = np.zeros_like(out), np.zeros_like(out)
     for s in range(len(kv_len)):
         r0, r1 = max(0, q_start[s]), min(len(q), q_start[s + 1])
         n = r1 - r0
@@ -111,5 +111,5 @@ def attend(q, k, v, q_start, kv_len, table, scale, causal, window, out):
                 x = kk @ q[r0 + i, h].astype(np.float64) * scale
                 p = np.exp(x - x.max())
                 p /= p.sum()
-                out[r0 + i, h], mag[r0 + i, h] = p @ vv, p @ np.abs(vv)
-    return out, mag
+                out[r0 + i, h], mag[r0 + i, h], total[r0 + i, h] = p @ vv, p @ np.abs(vv), np.abs(vv).sum(0)
+    return out, mag, total
