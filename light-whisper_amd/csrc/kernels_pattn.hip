@@ -118,24 +118,30 @@ __device__ __forceinline__ void load_words(uint32_t (&d)[N], const uint8_t* p) {
     }
 }
 
-// keys t0 .. t0 + 15 of sub-tile u, from their page's blocks
+// tokens t0 .. t0 + 15 of a page's block into sub-tile u
 template <int HD, int CT>
-__device__ __forceinline__ void load_sub(Slice<HD, CT>& s, int u, const uint8_t* kb, const uint8_t* vb, int t0,
-                                         uint32_t codes, int lane) {
+__device__ __forceinline__ void load_k(Slice<HD, CT>& s, int u, const uint8_t* kb, int t0, uint32_t codes, int lane) {
     const int n = lane & 15, kg = lane >> 4;
-    constexpr int ND = HD / 16;
     if constexpr (CT == T_MXFP4) {
         load_words(s.k[u], kb + t0 * (HD / 2) + n * (HD / 2) + kg * (HD / 8));
-        load_words(s.v[u], vb + t0 * (HD / 2) + lane * (2 * ND));
         const uint8_t* ks = kb + codes + (t0 + n) * (HD / 32);
         if constexpr (HD == 64) s.ks[u][0] = *(const uint16_t*)ks;
         else if constexpr (HD == 128) s.ks[u][0] = *(const uint32_t*)ks;
         else load_words(s.ks[u], ks);
-        s.vs[u] = *(const uint32_t*)(vb + codes + t0 * (HD / 32) + (n * ND / 32) * 16 + 4 * kg);
     } else {
         const uint8_t* kr = kb + (t0 + n) * (HD * 2) + kg * 16;
 #pragma unroll
         for (int kk = 0; kk < HD / 32; kk++) s.k[u][kk] = *(const u32x4*)(kr + kk * 64);
+    }
+}
+template <int HD, int CT>
+__device__ __forceinline__ void load_v(Slice<HD, CT>& s, int u, const uint8_t* vb, int t0, uint32_t codes, int lane) {
+    const int n = lane & 15, kg = lane >> 4;
+    constexpr int ND = HD / 16;
+    if constexpr (CT == T_MXFP4) {
+        load_words(s.v[u], vb + t0 * (HD / 2) + lane * (2 * ND));
+        s.vs[u] = *(const uint32_t*)(vb + codes + t0 * (HD / 32) + (n * ND / 32) * 16 + 4 * kg);
+    } else {
         const uint8_t* vr = vb + (t0 + 4 * kg) * (HD * 2) + n * (ND * 2);
 #pragma unroll
         for (int j = 0; j < 4; j++) {
@@ -153,8 +159,13 @@ __device__ __forceinline__ void load_sub(Slice<HD, CT>& s, int u, const uint8_t*
 }
 
 // Vᵀ operands of the dims ND·m + 2 b (t0) and + 2 b + 1 (t1): register p holds the lane's keys 2 p, 2 p + 1
-template <int HD, int CT, int QT>
+// (ANEW: not to be computed ahead of a loop that asks for them each time)
+template <int HD, int CT, int QT, bool ANEW = false>
 __device__ __forceinline__ void pair_v(const Slice<HD, CT>& s, int b, u32x4& t0, u32x4& t1) {
+    auto at = [](uint32_t v) {
+        if (ANEW) asm volatile("" : "+v"(v));
+        return v;
+    };
     constexpr int ND = HD / 16;
 #pragma unroll
     for (int p = 0; p < 4; p++) {
@@ -164,14 +175,14 @@ __device__ __forceinline__ void pair_v(const Slice<HD, CT>& s, int b, u32x4& t0,
             const float s0 = __uint_as_float(((s.vs[u] >> (8 * j)) & 255) << 23);
             const float s1 = __uint_as_float(((s.vs[u] >> (8 * j + 8)) & 255) << 23);
             const int i0 = j * (ND / 2) + b, i1 = (j + 1) * (ND / 2) + b;
-            x = fp4_pair<QT>(s.v[u][i0 / 4], s0, i0 % 4);
-            y = fp4_pair<QT>(s.v[u][i1 / 4], s1, i1 % 4);
+            x = fp4_pair<QT>(at(s.v[u][i0 / 4]), s0, i0 % 4);
+            y = fp4_pair<QT>(at(s.v[u][i1 / 4]), s1, i1 % 4);
         } else if constexpr (ND == 8) {
-            x = s.v[2 * p][b], y = s.v[2 * p + 1][b];
+            x = at(s.v[2 * p][b]), y = at(s.v[2 * p + 1][b]);
         } else if constexpr (ND == 16) {
-            x = s.v[4 * p + b / 4][b % 4], y = s.v[4 * p + 2 + b / 4][b % 4];
+            x = at(s.v[4 * p + b / 4][b % 4]), y = at(s.v[4 * p + 2 + b / 4][b % 4]);
         } else {
-            x = s.v[p][b], y = s.v[p][2 + b];
+            x = at(s.v[p][b]), y = at(s.v[p][2 + b]);
         }
         t0[p] = lo16(x, y);
         t1[p] = hi16(x, y);
@@ -238,7 +249,9 @@ __global__ __launch_bounds__(256, HD == 256 && CT != T_MXFP4 ? 1 : 2) void k_pag
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, n = lane & 15, kg = lane >> 4;
     const int G = a.nh / c.nkv;
     const uint32_t codes = (HD / 2) << c.page_shift;
-    const float sc = a.scale * 1.44269504088896340736f;
+    // a negative scale goes into q's signs; a zero one is the smallest number, so that −∞ of a masked key stays −∞
+    const float sc = fmaxf(fabsf(a.scale) * 1.44269504088896340736f, 1.17549435e-38f);
+    const uint32_t q_sign = a.scale < 0.f ? 0x80008000u : 0u;
 
     // ---- the list: tiles of every sequence, and where this workgroup's begin
     auto tiles_of = [&](const SeqWork& x) {   // key tiles of one item; an item without keys has one, which writes zeros
@@ -310,6 +323,8 @@ __global__ __launch_bounds__(256, HD == 256 && CT != T_MXFP4 ? 1 : 2) void k_pag
 #pragma unroll
                     for (int i = 0; i < 4; i++)
                         qf[kk][i] = qp[32 * kk + 2 * i] | (uint32_t)qp[32 * kk + 2 * i + 1] << 16;
+#pragma unroll
+                for (int i = 0; i < 4; i++) qf[kk][i] ^= q_sign;
             }
         }
 
@@ -324,149 +339,159 @@ __global__ __launch_bounds__(256, HD == 256 && CT != T_MXFP4 ? 1 : 2) void k_pag
         ids(0, id0, id1);
 
         f32x4 acc[ND];
+        float m, l;
+        auto clear = [&] {
 #pragma unroll
-        for (int i = 0; i < ND; i++) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-        float m = kNone, l = 0.f;
-
-        // loads of slice i; which of its sub-tiles have a page
-        auto load = [&](int i, Slice<HD, CT>& s) -> int {
-            const int key = key0 + i * kTileKeys + w * 32;
-            int have = 0;
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-                const int id = __builtin_amdgcn_readlane(u ? id1 : id0, i & 63);
-                const bool ok = (unsigned)id < (unsigned)c.n_pages && key + 16 * u < x.len;
-                const int64_t blk = ((int64_t)(ok ? id : 0) * c.nkv + kvh) * c.block_bytes;
-                if (ok) load_sub<HD, CT>(s, u, c.k + blk, c.v + blk, (key + 16 * u) & ((1 << c.page_shift) - 1), codes, lane);
-                have |= ok << u;
-            }
-            return have;
+            for (int i = 0; i < ND; i++) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+            m = kNone;
+            l = 0.f;
         };
-        auto compute = [&](int i, Slice<HD, CT>& s, int have) {
-            if (!have) return;
-            const int key = key0 + i * kTileKeys + w * 32;
-            const bool whole = have == 3 && key >= all_lo && key + 32 <= all_hi;
-            uint32_t see = 0xff;   // which of this lane's 8 keys its row sees
-            float p[8];
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-                f32x4 d = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int kk = 0; kk < KK; kk++) {
-                    if constexpr (CT == T_MXFP4) {
-                        const float f = __uint_as_float(((s.ks[u][kk / 4] >> (8 * (kk % 4))) & 255) << 23);
-                        const uint32_t wd = s.k[u][kk];
-                        const u32x4 kf = {fp4_pair<QT>(wd, f, 0), fp4_pair<QT>(wd, f, 1), fp4_pair<QT>(wd, f, 2),
-                                          fp4_pair<QT>(wd, f, 3)};
-                        d = mfma16<QT>(kf, qf[kk], d);
-                    } else {
-                        d = mfma16<QT>(s.k[u][kk], qf[kk], d);
-                    }
-                }
-#pragma unroll
-                for (int j = 0; j < 4; j++) p[4 * u + j] = d[j];
-            }
-            if constexpr (CT == T_MXFP4) {   // a scale byte of 255: the key is not a number
+        clear();
+
+        // where slice i lies: its two sub-tiles' blocks, and which have a page (the others load bytes that no row uses)
+        struct At {
+            int64_t b0, b1;
+            int t0, t1, have;
+        };
+        auto place = [&](int i) {
+            const int key = key0 + i * kTileKeys + w * 32, mask = (1 << c.page_shift) - 1;
+            const int d0 = __builtin_amdgcn_readlane(id0, i & 63), d1 = __builtin_amdgcn_readlane(id1, i & 63);
+            const bool ok0 = (unsigned)d0 < (unsigned)c.n_pages, ok1 = (unsigned)d1 < (unsigned)c.n_pages;
+            return At{((int64_t)(ok0 ? d0 : 0) * c.nkv + kvh) * c.block_bytes,
+                      ((int64_t)(ok1 ? d1 : 0) * c.nkv + kvh) * c.block_bytes, key & mask, (key + 16) & mask,
+                      (ok0 ? 1 : 0) | (ok1 ? 2 : 0)};
+        };
+
+        // ---- the segment's slices: the next slice's K is loaded into the registers of this one's as soon as its scores
+        // are there, and V's after the product
+        const int mine = max(0, min(seg, (x.len - key0 - 32 * w + kTileKeys - 1) / kTileKeys));   // with keys in them
+        bool careful = false;
+        for (bool again = mine > 0; again;) {
+            again = false;
+            clear();
+            Slice<HD, CT> s;
+            At pl = place(0);
+            load_k<HD, CT>(s, 0, c.k + pl.b0, pl.t0, codes, lane);
+            load_k<HD, CT>(s, 1, c.k + pl.b1, pl.t1, codes, lane);
+            load_v<HD, CT>(s, 0, c.v + pl.b0, pl.t0, codes, lane);
+            load_v<HD, CT>(s, 1, c.v + pl.b1, pl.t1, codes, lane);
+            for (int i = 0; i < mine; i++) {
+                const int key = key0 + i * kTileKeys + w * 32, have = pl.have;
+                const bool whole = have == 3 && key >= all_lo && key + 32 <= all_hi;
+                float p[8];
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
-                    bool nan = false;
+                    f32x4 d = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int kk = 0; kk < KK; kk++) nan |= ((s.ks[u][kk / 4] >> (8 * (kk % 4))) & 255) == 255;
-                    const uint64_t who = __ballot(nan && (have >> u & 1));   // lane n: key n
-                    if (who) {
+                    for (int kk = 0; kk < KK; kk++) {
+                        if constexpr (CT == T_MXFP4) {
+                            const float f = __uint_as_float(((s.ks[u][kk / 4] >> (8 * (kk % 4))) & 255) << 23);
+                            const uint32_t wd = s.k[u][kk];
+                            const u32x4 kf = {fp4_pair<QT>(wd, f, 0), fp4_pair<QT>(wd, f, 1), fp4_pair<QT>(wd, f, 2),
+                                              fp4_pair<QT>(wd, f, 3)};
+                            d = mfma16<QT>(kf, qf[kk], d);
+                        } else {
+                            d = mfma16<QT>(s.k[u][kk], qf[kk], d);
+                        }
+                    }
 #pragma unroll
-                        for (int j = 0; j < 4; j++)
-                            if (who >> (4 * kg + j) & 1) p[4 * u + j] = __uint_as_float(0x7fc00000u);
+                    for (int j = 0; j < 4; j++) p[4 * u + j] = d[j];
+                }
+                if constexpr (CT == T_MXFP4) {   // a scale byte of 255: the key (lane n's) is not a number
+                    bool nan[2];
+#pragma unroll
+                    for (int u = 0; u < 2; u++) {
+                        nan[u] = nan_scale(HD == 64 ? s.ks[u][0] & 0xffffu : s.ks[u][0]);
+                        if constexpr (HD == 256) nan[u] |= nan_scale(s.ks[u][1]);
+                    }
+                    if (__any(nan[0] || nan[1])) {
+#pragma unroll
+                        for (int u = 0; u < 2; u++) {
+                            const uint64_t who = __ballot(nan[u]);
+#pragma unroll
+                            for (int j = 0; j < 4; j++)
+                                if (who >> (4 * kg + j) & 1) p[4 * u + j] = __uint_as_float(0x7fc00000u);
+                        }
                     }
                 }
-            }
-            if (!whole) {
-                see = 0;
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const int kj = key + 16 * (j >> 2) + 4 * kg + (j & 3);
-                    if ((have >> (j >> 2) & 1) && kj >= lo && kj < hi) see |= 1u << j;
+                if (i + 1 < mine) {
+                    if (((i + 1) & 63) == 0) ids(i + 1, id0, id1);
+                    pl = place(i + 1);
+                    load_k<HD, CT>(s, 0, c.k + pl.b0, pl.t0, codes, lane);
+                    load_k<HD, CT>(s, 1, c.k + pl.b1, pl.t1, codes, lane);
                 }
-            }
-            float mx = kNone;
+                uint32_t see = 0xff;   // which of this lane's 8 keys its row sees
+                if (!whole) {
+                    see = 0;
+                    uint32_t real = 0;   // … and which any row may
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                p[j] *= sc;
-                if (!whole && !(see >> j & 1)) p[j] = -INFINITY;
-                mx = fmaxf(mx, p[j]);
-            }
-            if (__any(mx > m + kSlack)) {   // some row's maximum rose: move every row to its own
-                mx = fmaxf(mx, __shfl_xor(mx, 16));
-                mx = fmaxf(mx, __shfl_xor(mx, 32));
-                const float mn = fmaxf(m, mx), al = exp2f(m - mn);
-                m = mn;
-                l *= al;
-#pragma unroll
-                for (int t2 = 0; t2 < ND; t2++) acc[t2] *= al;
-            }
-            u32x4 pf;
-#pragma unroll
-            for (int j = 0; j < 8; j++) p[j] = exp2f(p[j] - (m - kUp));
-#pragma unroll
-            for (int j = 0; j < 4; j++) pf[j] = pack2<QT>(p[2 * j], p[2 * j + 1]);
-#pragma unroll
-            for (int j = 0; j < 8; j++) l += p[j];
-            bool odd_v = CT == T_MXFP4 && __any(v_not_finite<HD, CT, QT>(s));
-            if (!whole) {
-                // 0 · V is no zero where V is no number: drop what no row may use (behind the last key, no page)
-                uint32_t real = 0;
-#pragma unroll
-                for (int j = 0; j < 8; j++)
-                    if ((have >> (j >> 2) & 1) && key + 16 * (j >> 2) + 4 * kg + (j & 3) < x.len) real |= 1u << j;
-                zero_keys<HD, CT>(s, real);
-                odd_v = __any(v_not_finite<HD, CT, QT>(s));
-            }
-            if (!odd_v) {
-#pragma unroll
-                for (int b = 0; b < ND / 2; b++) {
-                    u32x4 v0, v1;
-                    pair_v<HD, CT, QT>(s, b, v0, v1);
-                    acc[2 * b] = mfma16<QT>(v0, pf, acc[2 * b]);
-                    acc[2 * b + 1] = mfma16<QT>(v1, pf, acc[2 * b + 1]);
+                    for (int j = 0; j < 8; j++) {
+                        const int kj = key + 16 * (j >> 2) + 4 * kg + (j & 3);
+                        const bool h = have >> (j >> 2) & 1;
+                        if (h && kj >= lo && kj < hi) see |= 1u << j;
+                        else p[j] = -INFINITY;
+                        if (h && kj < x.len) real |= 1u << j;
+                    }
+                    zero_keys<HD, CT>(s, real);
                 }
-            } else {
-                // … and where rows see different keys and such a V is among them, take the rows one by one
-                for (int n0 = 0; n0 < nrow; n0++) {
-                    const uint32_t sees = __shfl(see, 16 * kg + n0);
+                if ((!whole || CT == T_MXFP4) && !careful && __any(v_not_finite<HD, CT, QT>(s))) {
+                    // 0 · V is no zero where V is no number: from the start again, with the rows one by one
+                    careful = again = true;
+                    ids(0, id0, id1);
+                    break;
+                }
+                float mx = fmaxf(fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3])), fmaxf(fmaxf(p[4], p[5]), fmaxf(p[6], p[7])));
+                mx *= sc;
+                if (__any(mx > m + kSlack)) {   // some row's maximum rose: move every row to its own
+                    mx = fmaxf(mx, __shfl_xor(mx, 16));
+                    mx = fmaxf(mx, __shfl_xor(mx, 32));
+                    const float mn = fmaxf(m, mx), al = __builtin_amdgcn_exp2f(m - mn);
+                    m = mn;
+                    l *= al;
+#pragma unroll
+                    for (int t2 = 0; t2 < ND; t2++) acc[t2] *= al;
+                }
+                u32x4 pf;
+                const float mk = kUp - m;
+#pragma unroll
+                for (int j = 0; j < 8; j++) p[j] = __builtin_amdgcn_exp2f(fmaf(p[j], sc, mk));
+#pragma unroll
+                for (int j = 0; j < 4; j++) pf[j] = pack2<QT>(p[2 * j], p[2 * j + 1]);
+                l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+                if (!careful) {
 #pragma unroll
                     for (int b = 0; b < ND / 2; b++) {
                         u32x4 v0, v1;
                         pair_v<HD, CT, QT>(s, b, v0, v1);
+                        acc[2 * b] = mfma16<QT>(v0, pf, acc[2 * b]);
+                        acc[2 * b + 1] = mfma16<QT>(v1, pf, acc[2 * b + 1]);
+                    }
+                } else {
+                    for (int n0 = 0; n0 < nrow; n0++) {
+                        const uint32_t sees = __shfl(see, 16 * kg + n0);
 #pragma unroll
-                        for (int pr = 0; pr < 4; pr++) {
-                            if constexpr (CT == T_MXFP4) {   // a scale byte of 255 stands for NaN
-                                const uint32_t two = s.vs[pr / 2] >> (16 * (pr & 1));
-                                const uint32_t nan = ((two & 255) == 255 ? 0x7fffu : 0u) | ((two >> 8 & 255) == 255 ? 0x7fff0000u : 0u);
-                                v0[pr] |= nan, v1[pr] |= nan;
+                        for (int b = 0; b < ND / 2; b++) {
+                            u32x4 v0, v1;
+                            pair_v<HD, CT, QT, true>(s, b, v0, v1);
+#pragma unroll
+                            for (int pr = 0; pr < 4; pr++) {
+                                if constexpr (CT == T_MXFP4) {   // a scale byte of 255 stands for NaN
+                                    const uint32_t two = s.vs[pr / 2] >> (16 * (pr & 1));
+                                    const uint32_t nan = ((two & 255) == 255 ? 0x7fffu : 0u) | ((two >> 8 & 255) == 255 ? 0x7fff0000u : 0u);
+                                    v0[pr] |= nan, v1[pr] |= nan;
+                                }
+                                const uint32_t mask = (sees >> (2 * pr) & 1 ? 0xffffu : 0u) | (sees >> (2 * pr + 1) & 1 ? 0xffff0000u : 0u);
+                                v0[pr] &= mask, v1[pr] &= mask;
                             }
-                            const uint32_t mask = (sees >> (2 * pr) & 1 ? 0xffffu : 0u) | (sees >> (2 * pr + 1) & 1 ? 0xffff0000u : 0u);
-                            v0[pr] &= mask, v1[pr] &= mask;
+                            const f32x4 d0 = mfma16<QT>(v0, pf, acc[2 * b]), d1 = mfma16<QT>(v1, pf, acc[2 * b + 1]);
+                            if (n == n0) acc[2 * b] = d0, acc[2 * b + 1] = d1;
                         }
-                        const f32x4 d0 = mfma16<QT>(v0, pf, acc[2 * b]), d1 = mfma16<QT>(v1, pf, acc[2 * b + 1]);
-                        if (n == n0) acc[2 * b] = d0, acc[2 * b + 1] = d1;
                     }
                 }
-            }
-        };
-
-        // ---- the segment's slices, the next one's loads in flight behind each
-        {
-            Slice<HD, CT> sa{}, sb{};
-            int ha = load(0, sa), hb = 0;
-            for (int i = 0; i < seg; i += 2) {
-                if (i + 1 < seg) hb = load(i + 1, sb);
-                compute(i, sa, ha);
-                if (i + 1 >= seg) break;
-                if (i + 2 < seg) {
-                    if (((i + 2) & 63) == 0) ids(i + 2, id0, id1);
-                    ha = load(i + 2, sa);
+                if (i + 1 < mine) {
+                    load_v<HD, CT>(s, 0, c.v + pl.b0, pl.t0, codes, lane);
+                    load_v<HD, CT>(s, 1, c.v + pl.b1, pl.t1, codes, lane);
                 }
-                compute(i + 1, sb, hb);
             }
         }
 
@@ -488,7 +513,7 @@ __global__ __launch_bounds__(256, HD == 256 && CT != T_MXFP4 ? 1 : 2) void k_pag
         if (n < nrow) {
 #pragma unroll
             for (int v = 0; v < 4; v++) {
-                const float f = exp2f(s_m[v][n] - M);
+                const float f = __builtin_amdgcn_exp2f(s_m[v][n] - M);
                 Lsum = fmaf(s_l[v][n], f, Lsum);
 #pragma unroll
                 for (int t2 = 0; t2 < ND; t2++) out[t2] = fmaf(s_acc[v][t2 * 4 + w][lane], f, out[t2]);
@@ -546,7 +571,7 @@ __global__ __launch_bounds__(256, HD == 256 && CT != T_MXFP4 ? 1 : 2) void k_pag
 #pragma unroll
                         for (int u = 0; u < U; u++) {
                             if (p0 + u * step >= pieces) continue;
-                            const float mn = fmaxf(M, pm[u]), f0 = exp2f(M - mn), f1 = exp2f(pm[u] - mn);
+                            const float mn = fmaxf(M, pm[u]), f0 = __builtin_amdgcn_exp2f(M - mn), f1 = __builtin_amdgcn_exp2f(pm[u] - mn);
                             M = mn;
                             Lsum = Lsum * f0 + pl[u] * f1;
 #pragma unroll
@@ -556,7 +581,7 @@ __global__ __launch_bounds__(256, HD == 256 && CT != T_MXFP4 ? 1 : 2) void k_pag
                 }
                 for (int s = R; s < 16; s <<= 1) {
                     const float om = __shfl_xor(M, s), ol = __shfl_xor(Lsum, s);
-                    const float mn = fmaxf(M, om), f0 = exp2f(M - mn), f1 = exp2f(om - mn);
+                    const float mn = fmaxf(M, om), f0 = __builtin_amdgcn_exp2f(M - mn), f1 = __builtin_amdgcn_exp2f(om - mn);
                     Lsum = Lsum * f0 + ol * f1;
                     M = mn;
 #pragma unroll
@@ -617,9 +642,11 @@ static void launch(const KvPages& c, const AttnArgs& a, const void* q, int64_t l
                                                   o_vec);
 }
 
-void paged_attention(const KvPages& c, const AttnArgs& a, const void* q, int64_t ldq, const int* q_start,
+void paged_attention(const KvPages& cache, const AttnArgs& a, const void* q, int64_t ldq, const int* q_start,
                      const int* kv_len, int rows, void* o, int64_t ldo, void* ws, hipStream_t s) {
-    if (rows <= 0 || c.n_seq <= 0) return;
+    if (rows <= 0 || cache.n_seq <= 0) return;
+    KvPages c = cache;
+    if (c.n_pages == 0) c.max_pages = 0;   // no page to read from: no keys
     auto by_types = [&](auto hd) {
         constexpr int HD = decltype(hd)::value;
         if (c.type == T_F16) launch<HD, T_F16, T_F16>(c, a, q, ldq, q_start, kv_len, rows, o, ldo, ws, s);
