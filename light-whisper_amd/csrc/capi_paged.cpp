@@ -98,7 +98,8 @@ AttnArgs attn_of(const KvPages& c, const qasr_paged_attn* a) {
                "paged_attention: o must be of q's type or f32");
     QASR_CHECK(isfinite(a->scale), QASR_E_INVALID, "paged_attention: scale must be finite");
     QASR_CHECK(a->window >= 0 && a->max_q >= 0 && a->max_kv >= 0, QASR_E_INVALID, "paged_attention: negative size");
-    return AttnArgs{a->n_heads, a->q_type, a->o_type, a->causal != 0, a->window, a->max_q, a->max_kv, a->scale};
+    // no position lies further than 2^30 from another
+    return AttnArgs{a->n_heads, a->q_type, a->o_type, a->causal != 0, a->window < 1 << 30 ? a->window : 1 << 30, a->max_q, a->max_kv, a->scale};
 }
 
 }  // namespace

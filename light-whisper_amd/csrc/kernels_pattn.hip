@@ -22,6 +22,8 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kTileKeys = 128;   // keys of one workgroup step: 32 for each of its 4 waves
 constexpr int kSplitWgs = 1024;  // workgroups at most (what the scratch is sized for)
+// workgroups that a CU holds by their registers
+constexpr int wgs_per_cu(int hd, int ct) { return ct == T_MXFP4 ? (hd == 256 ? 2 : 3) : hd == 256 ? 1 : 2; }
 // weights are exp2(s − m + kUp), m at most kSlack below the running maximum: at most 2^15 in f16, and its normal range
 // reaches 26 bits further down
 constexpr float kSlack = 3.f, kUp = 12.f;
@@ -87,7 +89,7 @@ __device__ __forceinline__ SeqWork seq_work(const KvPages& c, const AttnArgs& a,
     w.nq = max(min(q_start[s + 1], rows) - w.row0, 0);
     w.len = (int)min((int64_t)max(kv_len[s], 0), (int64_t)c.max_pages << c.page_shift);
     // the first row's window starts furthest left; with len < nq its position is negative
-    w.lo = a.window > 0 ? min(max((int64_t)w.len - w.nq - a.window + 1, (int64_t)0), (int64_t)w.len) : 0;
+    w.lo = a.window > 0 ? max(w.len - w.nq - a.window + 1, 0) : 0;
     return w;
 }
 
@@ -103,15 +105,25 @@ struct Slice<HD, T_MXFP4> {
     uint32_t ks[2][HD == 256 ? 2 : 1], vs[2];
 };
 
+// One block of a page as a buffer: 32-bit lane offsets, and nothing past the block is ever read
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t block_rsrc(const uint8_t* base, uint32_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base), (short)0, (int)bytes, 0x00020000);
+}
+__device__ __forceinline__ u32x4 load4(__amdgpu_buffer_rsrc_t r, uint32_t lane_off, uint32_t off) {
+    return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, lane_off, off, 0));
+}
+__device__ __forceinline__ u32x2 load2(__amdgpu_buffer_rsrc_t r, uint32_t lane_off, uint32_t off) {
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, lane_off, off, 0));
+}
 template <int N>
-__device__ __forceinline__ void load_words(uint32_t (&d)[N], const uint8_t* p) {
+__device__ __forceinline__ void load_words(uint32_t (&d)[N], __amdgpu_buffer_rsrc_t r, uint32_t lane_off, uint32_t off) {
     if constexpr (N == 2) {
-        const u32x2 t = *(const u32x2*)p;
+        const u32x2 t = load2(r, lane_off, off);
         d[0] = t[0], d[1] = t[1];
     } else {
 #pragma unroll
         for (int i = 0; i < N / 4; i++) {
-            const u32x4 t = *(const u32x4*)(p + 16 * i);
+            const u32x4 t = load4(r, lane_off + 16 * i, off);
 #pragma unroll
             for (int j = 0; j < 4; j++) d[4 * i + j] = t[j];
         }
@@ -120,37 +132,36 @@ __device__ __forceinline__ void load_words(uint32_t (&d)[N], const uint8_t* p) {
 
 // tokens t0 .. t0 + 15 of a page's block into sub-tile u
 template <int HD, int CT>
-__device__ __forceinline__ void load_k(Slice<HD, CT>& s, int u, const uint8_t* kb, int t0, uint32_t codes, int lane) {
-    const int n = lane & 15, kg = lane >> 4;
+__device__ __forceinline__ void load_k(Slice<HD, CT>& s, int u, __amdgpu_buffer_rsrc_t kb, int t0, uint32_t codes, int n,
+                                       int kg) {
     if constexpr (CT == T_MXFP4) {
-        load_words(s.k[u], kb + t0 * (HD / 2) + n * (HD / 2) + kg * (HD / 8));
-        const uint8_t* ks = kb + codes + (t0 + n) * (HD / 32);
-        if constexpr (HD == 64) s.ks[u][0] = *(const uint16_t*)ks;
-        else if constexpr (HD == 128) s.ks[u][0] = *(const uint32_t*)ks;
-        else load_words(s.ks[u], ks);
+        load_words(s.k[u], kb, n * (HD / 2) + kg * (HD / 8), t0 * (HD / 2));
+        const uint32_t ks = codes + t0 * (HD / 32);
+        if constexpr (HD == 64) s.ks[u][0] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(kb, n * 2, ks, 0);
+        else if constexpr (HD == 128) s.ks[u][0] = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(kb, n * 4, ks, 0);
+        else load_words(s.ks[u], kb, n * 8, ks);
     } else {
-        const uint8_t* kr = kb + (t0 + n) * (HD * 2) + kg * 16;
 #pragma unroll
-        for (int kk = 0; kk < HD / 32; kk++) s.k[u][kk] = *(const u32x4*)(kr + kk * 64);
+        for (int kk = 0; kk < HD / 32; kk++) s.k[u][kk] = load4(kb, n * (HD * 2) + kg * 16 + kk * 64, t0 * (HD * 2));
     }
 }
 template <int HD, int CT>
-__device__ __forceinline__ void load_v(Slice<HD, CT>& s, int u, const uint8_t* vb, int t0, uint32_t codes, int lane) {
-    const int n = lane & 15, kg = lane >> 4;
+__device__ __forceinline__ void load_v(Slice<HD, CT>& s, int u, __amdgpu_buffer_rsrc_t vb, int t0, uint32_t codes, int n,
+                                       int kg) {
     constexpr int ND = HD / 16;
     if constexpr (CT == T_MXFP4) {
-        load_words(s.v[u], vb + t0 * (HD / 2) + lane * (2 * ND));
-        s.vs[u] = *(const uint32_t*)(vb + codes + t0 * (HD / 32) + (n * ND / 32) * 16 + 4 * kg);
+        load_words(s.v[u], vb, (16 * kg + n) * (2 * ND), t0 * (HD / 2));
+        s.vs[u] = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(vb, (n * ND / 32) * 16 + 4 * kg, codes + t0 * (HD / 32), 0);
     } else {
-        const uint8_t* vr = vb + (t0 + 4 * kg) * (HD * 2) + n * (ND * 2);
+        const uint32_t vr = 4 * kg * (HD * 2) + n * (ND * 2), off = t0 * (HD * 2);
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            if constexpr (ND == 8) s.v[4 * u + j] = *(const u32x4*)(vr + j * (HD * 2));
+            if constexpr (ND == 8) s.v[4 * u + j] = load4(vb, vr + j * (HD * 2), off);
             else if constexpr (ND == 16) {
-                s.v[8 * u + 2 * j] = *(const u32x4*)(vr + j * (HD * 2));
-                s.v[8 * u + 2 * j + 1] = *(const u32x4*)(vr + j * (HD * 2) + 16);
+                s.v[8 * u + 2 * j] = load4(vb, vr + j * (HD * 2), off);
+                s.v[8 * u + 2 * j + 1] = load4(vb, vr + j * (HD * 2) + 16, off);
             } else {
-                const u32x2 t = *(const u32x2*)(vr + j * (HD * 2));
+                const u32x2 t = load2(vb, vr + j * (HD * 2), off);
                 s.v[2 * u + j / 2][2 * (j & 1)] = t[0];
                 s.v[2 * u + j / 2][2 * (j & 1) + 1] = t[1];
             }
@@ -211,14 +222,18 @@ __device__ __forceinline__ void zero_keys(Slice<HD, CT>& s, uint32_t keep) {
         }
     }
 }
-__device__ __forceinline__ bool nan_scale(uint32_t b) {   // one of four scale bytes is 255
-    return (b & 255) == 255 || (b >> 8 & 255) == 255 || (b >> 16 & 255) == 255 || b >> 24 == 255;
+// not 0 where one of four scale bytes is 255: it alone has its two highest bits set (the others are 104 .. 140)
+__device__ __forceinline__ uint32_t nan_scale(uint32_t b) { return b & (b << 1) & 0x80808080u; }
+// a value that the compiler takes for new here: what follows from it is not computed ahead and held in registers
+__device__ __forceinline__ int anew(int v) {
+    asm volatile("" : "+v"(v));
+    return v;
 }
 // some V of the lane's keys is an infinity or NaN
 template <int HD, int CT, int QT>
 __device__ __forceinline__ bool v_not_finite(const Slice<HD, CT>& s) {
     if constexpr (CT == T_MXFP4) {
-        return nan_scale(s.vs[0]) || nan_scale(s.vs[1]);
+        return (nan_scale(s.vs[0]) | nan_scale(s.vs[1])) != 0;
     } else {
         constexpr uint32_t e = QT == T_F16 ? 0x7c00u : 0x7f80u;
         bool bad = false;
@@ -237,7 +252,7 @@ __device__ __forceinline__ bool v_not_finite(const Slice<HD, CT>& s) {
 // (m, l, Oᵀ) in the scratch, and the last of the item's workgroups to arrive adds them up in their order (the result does
 // not depend on who is last).  Slot 0 of a workgroup: the item began in an earlier one; slot 1: it goes on in a later one.
 template <int HD, int CT, int QT>
-__global__ __launch_bounds__(256, HD == 256 && CT != T_MXFP4 ? 1 : 2) void k_paged_attn(KvPages c, AttnArgs a, const void* __restrict__ q, int64_t ldq,
+__global__ __launch_bounds__(256, wgs_per_cu(HD, CT)) void k_paged_attn(KvPages c, AttnArgs a, const void* __restrict__ q, int64_t ldq,
                                                        const int* __restrict__ q_start, const int* __restrict__ kv_len,
                                                        int rows, void* __restrict__ o, int64_t ldo, float* part,
                                                        unsigned* cnt, int min_tiles, int q_vec, int o_vec) {
@@ -246,7 +261,7 @@ __global__ __launch_bounds__(256, HD == 256 && CT != T_MXFP4 ? 1 : 2) void k_pag
     __shared__ float s_acc[4][ND * 4][LANES];
     __shared__ float s_m[4][16], s_l[4][16];
     __shared__ int s_last;
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, n = lane & 15, kg = lane >> 4;
+    const int lane = threadIdx.x & 63, w = uniform(threadIdx.x >> 6);
     const int G = a.nh / c.nkv;
     const uint32_t codes = (HD / 2) << c.page_shift;
     // a negative scale goes into q's signs; a zero one is the smallest number, so that −∞ of a masked key stays −∞
@@ -285,6 +300,10 @@ __global__ __launch_bounds__(256, HD == 256 && CT != T_MXFP4 ? 1 : 2) void k_pag
     }
 
     while (t < t_end) {
+        // what follows from the lane's place is computed anew for each segment: held over the loop it takes the registers
+        // of a third of the waves
+        const int ln = anew(lane);
+        const int n = ln & 15, kg = ln >> 4;
         // ---- the segment that tile t begins
         while (t >= before + __builtin_amdgcn_readlane(scan, 63)) {
             before += __builtin_amdgcn_readlane(scan, 63);
@@ -303,19 +322,23 @@ __global__ __launch_bounds__(256, HD == 256 && CT != T_MXFP4 ? 1 : 2) void k_pag
         const int nrow = min(16, x.nq * G - rt * 16);
 
         // ---- this lane's row: its keys [lo, hi) and its q
-        const int r = rt * 16 + min(n, nrow - 1), tok = r / G, head = kvh * G + r % G;
-        const int64_t row = x.row0 + tok;
-        const int64_t at = (int64_t)x.len - x.nq + tok;
-        const int hi = a.causal ? (int)min((int64_t)x.len, at + 1) : x.len;
-        const int lo = a.window > 0 ? (int)max((int64_t)0, at - a.window + 1) : 0;
+        // (positions: lengths are at most 2^30, row counts below 2^31, so differences fit; windows are cut to 2^30)
+        auto row_of = [&](int nn, int& tok, int& head) {
+            const int r = rt * 16 + min(nn, nrow - 1);
+            tok = r / G;
+            head = kvh * G + r % G;
+        };
+        int tok, head;
+        row_of(n, tok, head);
+        const int p0 = x.len - x.nq, at = p0 + tok;
+        const int hi = a.causal ? min(x.len, at + 1) : x.len;
+        const int lo = a.window > 0 ? max(0, at - a.window + 1) : 0;
         // keys [all_lo, all_hi) are seen by every row of the tile
-        const int last_tok = (rt * 16 + nrow - 1) / G, first_tok = rt * 16 / G;
-        const int64_t p0 = (int64_t)x.len - x.nq + first_tok, p1 = (int64_t)x.len - x.nq + last_tok;
-        const int all_hi = a.causal ? (int)max((int64_t)0, min((int64_t)x.len, p0 + 1)) : x.len;
-        const int all_lo = a.window > 0 ? (int)max((int64_t)0, p1 - a.window + 1) : 0;
+        const int all_hi = a.causal ? max(0, min(x.len, p0 + rt * 16 / G + 1)) : x.len;
+        const int all_lo = a.window > 0 ? max(0, p0 + (rt * 16 + nrow - 1) / G - a.window + 1) : 0;
         u32x4 qf[KK];
         {
-            const uint16_t* qp = (const uint16_t*)q + row * ldq + (int64_t)head * HD + 8 * kg;
+            const uint16_t* qp = (const uint16_t*)q + (x.row0 + tok) * ldq + (int64_t)head * HD + 8 * kg;
 #pragma unroll
             for (int kk = 0; kk < KK; kk++) {
                 if (q_vec) qf[kk] = *(const u32x4*)(qp + 32 * kk);
@@ -371,10 +394,10 @@ __global__ __launch_bounds__(256, HD == 256 && CT != T_MXFP4 ? 1 : 2) void k_pag
             clear();
             Slice<HD, CT> s;
             At pl = place(0);
-            load_k<HD, CT>(s, 0, c.k + pl.b0, pl.t0, codes, lane);
-            load_k<HD, CT>(s, 1, c.k + pl.b1, pl.t1, codes, lane);
-            load_v<HD, CT>(s, 0, c.v + pl.b0, pl.t0, codes, lane);
-            load_v<HD, CT>(s, 1, c.v + pl.b1, pl.t1, codes, lane);
+            load_k<HD, CT>(s, 0, block_rsrc(c.k + pl.b0, c.block_bytes), pl.t0, codes, n, kg);
+            load_k<HD, CT>(s, 1, block_rsrc(c.k + pl.b1, c.block_bytes), pl.t1, codes, n, kg);
+            load_v<HD, CT>(s, 0, block_rsrc(c.v + pl.b0, c.block_bytes), pl.t0, codes, n, kg);
+            load_v<HD, CT>(s, 1, block_rsrc(c.v + pl.b1, c.block_bytes), pl.t1, codes, n, kg);
             for (int i = 0; i < mine; i++) {
                 const int key = key0 + i * kTileKeys + w * 32, have = pl.have;
                 const bool whole = have == 3 && key >= all_lo && key + 32 <= all_hi;
@@ -398,35 +421,37 @@ __global__ __launch_bounds__(256, HD == 256 && CT != T_MXFP4 ? 1 : 2) void k_pag
                     for (int j = 0; j < 4; j++) p[4 * u + j] = d[j];
                 }
                 if constexpr (CT == T_MXFP4) {   // a scale byte of 255: the key (lane n's) is not a number
-                    bool nan[2];
+                    uint32_t nan[2];
 #pragma unroll
                     for (int u = 0; u < 2; u++) {
-                        nan[u] = nan_scale(HD == 64 ? s.ks[u][0] & 0xffffu : s.ks[u][0]);
+                        nan[u] = nan_scale(s.ks[u][0]);
                         if constexpr (HD == 256) nan[u] |= nan_scale(s.ks[u][1]);
                     }
-                    if (__any(nan[0] || nan[1])) {
+                    if (__any((nan[0] | nan[1]) != 0)) {
+                        const int kq = 4 * anew(kg);
 #pragma unroll
                         for (int u = 0; u < 2; u++) {
-                            const uint64_t who = __ballot(nan[u]);
+                            const uint32_t who = (uint32_t)__ballot(nan[u] != 0) >> kq;
 #pragma unroll
                             for (int j = 0; j < 4; j++)
-                                if (who >> (4 * kg + j) & 1) p[4 * u + j] = __uint_as_float(0x7fc00000u);
+                                if (who >> j & 1) p[4 * u + j] = __uint_as_float(0x7fc00000u);
                         }
                     }
                 }
                 if (i + 1 < mine) {
                     if (((i + 1) & 63) == 0) ids(i + 1, id0, id1);
                     pl = place(i + 1);
-                    load_k<HD, CT>(s, 0, c.k + pl.b0, pl.t0, codes, lane);
-                    load_k<HD, CT>(s, 1, c.k + pl.b1, pl.t1, codes, lane);
+                    load_k<HD, CT>(s, 0, block_rsrc(c.k + pl.b0, c.block_bytes), pl.t0, codes, n, kg);
+                    load_k<HD, CT>(s, 1, block_rsrc(c.k + pl.b1, c.block_bytes), pl.t1, codes, n, kg);
                 }
                 uint32_t see = 0xff;   // which of this lane's 8 keys its row sees
                 if (!whole) {
                     see = 0;
                     uint32_t real = 0;   // … and which any row may
+                    const int k4 = key + 4 * anew(kg);
 #pragma unroll
                     for (int j = 0; j < 8; j++) {
-                        const int kj = key + 16 * (j >> 2) + 4 * kg + (j & 3);
+                        const int kj = k4 + 16 * (j >> 2) + (j & 3);
                         const bool h = have >> (j >> 2) & 1;
                         if (h && kj >= lo && kj < hi) see |= 1u << j;
                         else p[j] = -INFINITY;
@@ -489,8 +514,8 @@ __global__ __launch_bounds__(256, HD == 256 && CT != T_MXFP4 ? 1 : 2) void k_pag
                     }
                 }
                 if (i + 1 < mine) {
-                    load_v<HD, CT>(s, 0, c.v + pl.b0, pl.t0, codes, lane);
-                    load_v<HD, CT>(s, 1, c.v + pl.b1, pl.t1, codes, lane);
+                    load_v<HD, CT>(s, 0, block_rsrc(c.v + pl.b0, c.block_bytes), pl.t0, codes, n, kg);
+                    load_v<HD, CT>(s, 1, block_rsrc(c.v + pl.b1, c.block_bytes), pl.t1, codes, n, kg);
                 }
             }
         }
@@ -504,7 +529,7 @@ __global__ __launch_bounds__(256, HD == 256 && CT != T_MXFP4 ? 1 : 2) void k_pag
 #pragma unroll
             for (int t2 = 0; t2 < ND; t2++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) s_acc[w][t2 * 4 + i][lane] = acc[t2][i];
+                for (int i = 0; i < 4; i++) s_acc[w][t2 * 4 + i][ln] = acc[t2][i];
         }
         __syncthreads();
         float M = fmaxf(fmaxf(s_m[0][n], s_m[1][n]), fmaxf(s_m[2][n], s_m[3][n])), Lsum = 0.f, out[ND];
@@ -516,7 +541,7 @@ __global__ __launch_bounds__(256, HD == 256 && CT != T_MXFP4 ? 1 : 2) void k_pag
                 const float f = __builtin_amdgcn_exp2f(s_m[v][n] - M);
                 Lsum = fmaf(s_l[v][n], f, Lsum);
 #pragma unroll
-                for (int t2 = 0; t2 < ND; t2++) out[t2] = fmaf(s_acc[v][t2 * 4 + w][lane], f, out[t2]);
+                for (int t2 = 0; t2 < ND; t2++) out[t2] = fmaf(s_acc[v][t2 * 4 + w][ln], f, out[t2]);
             }
         }
         bool write = true;
@@ -596,7 +621,9 @@ __global__ __launch_bounds__(256, HD == 256 && CT != T_MXFP4 ? 1 : 2) void k_pag
             const float inv = Lsum == 0.f ? 0.f : 1.f / Lsum;
 #pragma unroll
             for (int t2 = 0; t2 < ND; t2++) out[t2] *= inv;
-            const int64_t at_o = row * ldo + (int64_t)head * HD + ND * (4 * kg + w);
+            int tok, head;
+            row_of(anew(n), tok, head);
+            const int64_t at_o = (x.row0 + tok) * ldo + (int64_t)head * HD + ND * (4 * kg + w);
             if (a.o_type == T_F32) {
                 float* op = (float*)o + at_o;
 #pragma unroll
@@ -634,7 +661,7 @@ static void launch(const KvPages& c, const AttnArgs& a, const void* q, int64_t l
     const int G = a.nh / c.nkv, min_tiles = 1;
     const int64_t items = ((int64_t)rows * G / 16 + c.n_seq) * c.nkv;   // at most
     const int64_t tiles = items * std::max<int64_t>(1, cdiv64(a.max_kv, kTileKeys));
-    const int grid = (int)std::min<int64_t>(512, std::max<int64_t>(1, cdiv64(tiles, min_tiles)));
+    const int grid = (int)std::min<int64_t>(256 * wgs_per_cu(HD, CT), std::max<int64_t>(1, cdiv64(tiles, min_tiles)));
     const int q_vec = ldq % 8 == 0 && ((uintptr_t)q & 15) == 0;
     const int o_vec = ldo % 4 == 0 && ((uintptr_t)o & 15) == 0;
     k_paged_attn<HD, CT, QT><<<grid, 256, 0, s>>>(c, a, q, ldq, q_start, kv_len, rows, o, ldo,
