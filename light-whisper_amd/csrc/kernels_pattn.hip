@@ -7,6 +7,7 @@
 //                (lane >> 4, j) stands for key 16 (j >> 2) + 4 (lane >> 4) + (j & 3), and V is loaded to match)
 // No K/V byte passes LDS: K rows are loaded in the A operand's layout; a lane loads hd/16 dims of its 8 keys of V and
 // pairs them key by key in registers (v_perm), which makes MFMA row m of tile t dim (hd/16) m + t.
+#include "lds_dma.h"
 #include "paged_dev.h"
 #include "wt.h"
 
@@ -14,6 +15,9 @@ namespace qasr {
 namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
@@ -35,6 +39,14 @@ __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
     else
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
+                                                       0);
+}
+template <int QT>
+__device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
+    if constexpr (QT == T_F16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
                                                        0);
 }
 // two f32 → a packed pair of QT, rounded to nearest even
@@ -245,6 +257,24 @@ __device__ __forceinline__ bool v_not_finite(const Slice<HD, CT>& s) {
     }
 }
 
+// four values of o
+template <int QT>
+__device__ __forceinline__ void store_out(void* o, int o_type, int64_t at, f32x4 v, int o_vec) {
+    if (o_type == T_F32) {
+        float* op = (float*)o + at;
+        if (o_vec) *(f32x4*)op = v;
+        else
+#pragma unroll
+            for (int i = 0; i < 4; i++) op[i] = v[i];
+    } else {
+        uint16_t* op = (uint16_t*)o + at;
+        const u32x2 d = {pack2<QT>(v[0], v[1]), pack2<QT>(v[2], v[3])};
+        if (o_vec) *(u32x2*)op = d;
+        else
+#pragma unroll
+            for (int i = 0; i < 4; i++) op[i] = (uint16_t)(d[i / 2] >> (16 * (i & 1)));
+    }
+}
 // ------------------------------------------------------------------------------------------------ few rows
 // One launch over every sequence: the work is the list of (sequence, 16-row tile, KV head) items, each ⌈keys / 128⌉ tiles
 // long; workgroup w takes tiles [w · per, (w + 1) · per) of the whole list, so lengths that differ a thousandfold load the
@@ -624,48 +654,452 @@ __global__ __launch_bounds__(256, wgs_per_cu(HD, CT)) void k_paged_attn(KvPages 
             int tok, head;
             row_of(anew(n), tok, head);
             const int64_t at_o = (x.row0 + tok) * ldo + (int64_t)head * HD + ND * (4 * kg + w);
-            if (a.o_type == T_F32) {
-                float* op = (float*)o + at_o;
 #pragma unroll
-                for (int t2 = 0; t2 < ND; t2 += 4) {
-                    if (o_vec) *(f32x4*)(op + t2) = f32x4{out[t2], out[t2 + 1], out[t2 + 2], out[t2 + 3]};
-                    else
-#pragma unroll
-                        for (int i = 0; i < 4; i++) op[t2 + i] = out[t2 + i];
-                }
-            } else {
-                uint16_t* op = (uint16_t*)o + at_o;
-#pragma unroll
-                for (int t2 = 0; t2 < ND; t2 += 4) {
-                    const u32x2 d = {pack2<QT>(out[t2], out[t2 + 1]), pack2<QT>(out[t2 + 2], out[t2 + 3])};
-                    if (o_vec) *(u32x2*)(op + t2) = d;
-                    else
-#pragma unroll
-                        for (int i = 0; i < 4; i++) op[t2 + i] = (uint16_t)(d[i / 2] >> (16 * (i & 1)));
-                }
-            }
+            for (int t2 = 0; t2 < ND; t2 += 4)
+                store_out<QT>(o, a.o_type, at_o + t2, f32x4{out[t2], out[t2 + 1], out[t2 + 2], out[t2 + 3]}, o_vec);
         }
         t += seg;
     }
 }
 
+
+// ------------------------------------------------------------------------------------------------ many rows
+// A workgroup takes 128 rows of one sequence and KV head, 32 for each of its 4 waves (v_mfma_f32_32x32x16, the same two
+// products: a lane holds 32 of 64 scores of one row), and walks the keys in tiles of 64 that all waves share through two
+// LDS buffers: tile t + 1 is on its way (LDS-DMA; 4-bit pages by registers, widened as they are stored) while t is used,
+// one barrier a tile.  Vᵀ comes out of LDS by transposing reads.  Rows of 16-byte chunks, chunk c of row r at c ^ swz(r):
+//   K  swz = r mod chunks: 8 neighbouring rows' chunks fall in 8 places
+//   V  swz = 4 (r mod 4) (head_dim 64: 4 (r / 2 mod 2)): the 4 rows × 64 bytes of a transposing read's half wave fall in
+//      the 16 places of 256 bytes
+// Work: items (sequence, 128 rows, KV head), the longest first, KV heads side by side (neighbouring workgroups go to
+// different XCDs: with 8 heads an XCD's L2 serves one).  Where the items are too few for the chip, `splits` workgroups
+// share one item's keys and the last to arrive joins their parts.
+constexpr int kRowBlock = 128, kPromptKeys = 64;
+
+template <int HD>
+__device__ __forceinline__ int k_swz(int row) { return row & (HD / 8 - 1); }
+template <int HD>
+__device__ __forceinline__ int v_swz(int row) { return HD == 64 ? (row & 2) << 1 : (row & 3) << 2; }
+
+template <int HD, int CT, int QT>
+__global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_paged_prompt(
+    KvPages c, AttnArgs a, const void* __restrict__ q, int64_t ldq, const int* __restrict__ q_start,
+    const int* __restrict__ kv_len, int rows, void* __restrict__ o, int64_t ldo, float* part, unsigned* cnt, int splits,
+    int q_vec, int o_vec) {
+    constexpr int KK = HD / 16, DT = HD / 32, CPR = HD / 8, ROW = HD * 2;
+    constexpr int kSlot = kRowBlock * (HD + 2);   // floats: Oᵀ as [wave][dim tile · 4 + i / 4][lane][4], then m, l per row
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    __shared__ int s_ok[2][4];
+    __shared__ uint64_t s_odd[4];
+    __shared__ int s_last;
+    constexpr int TILE = kPromptKeys * ROW;
+    uint8_t* const ldsK = lds;             // [2][TILE]
+    uint8_t* const ldsV = lds + 2 * TILE;  // [2][TILE]
+    const int lane = threadIdx.x & 63, w = uniform(threadIdx.x >> 6), n = lane & 31, h = lane >> 5;
+    const int G = a.nh / c.nkv;
+    const uint32_t codes = (HD / 2) << c.page_shift;
+    const float sc = fmaxf(fabsf(a.scale) * 1.44269504088896340736f, 1.17549435e-38f);   // as in k_paged_attn
+    const uint32_t q_sign = a.scale < 0.f ? 0x80008000u : 0u;
+
+    // ---- this workgroup's item
+    const int split = blockIdx.x % splits, item = blockIdx.x / splits;
+    const int kvh = item % c.nkv;
+    int blk = item / c.nkv;   // row block, counted over the sequences
+    SeqWork x{};
+    int seq = -1;
+    for (int s0 = 0; s0 < c.n_seq; s0 += 64) {
+        SeqWork my{};
+        if (s0 + lane < c.n_seq) my = seq_work(c, a, q_start, kv_len, rows, s0 + lane);
+        const int blocks = (my.nq * G + kRowBlock - 1) / kRowBlock, scan = wave_scan(blocks);
+        const int in = __builtin_amdgcn_readlane(scan, 63);
+        if (blk < in) {
+            const int sl = __popcll(__ballot(scan <= blk));
+            seq = s0 + sl;
+            x = SeqWork{__builtin_amdgcn_readlane(my.row0, sl), __builtin_amdgcn_readlane(my.nq, sl),
+                        __builtin_amdgcn_readlane(my.len, sl), __builtin_amdgcn_readlane(my.lo, sl)};
+            blk = __builtin_amdgcn_readlane(scan, sl) - 1 - blk;   // a sequence's last rows see the most keys: first
+            break;
+        }
+        blk -= in;
+    }
+    if (seq < 0) return;
+    const int row_base = blk * kRowBlock, nrow = min(kRowBlock, x.nq * G - row_base);   // rows r = token · G + g
+    // the keys that any row of the block sees, in tiles, and this workgroup's part of them
+    const int p0 = x.len - x.nq;
+    const int b_hi = a.causal ? max(0, min(x.len, p0 + (row_base + nrow - 1) / G + 1)) : x.len;
+    const int b_lo = a.window > 0 ? min(b_hi, max(0, p0 + row_base / G - a.window + 1)) : 0;
+    // … and those that every row sees
+    const int blk_hi = a.causal ? max(0, min(x.len, p0 + row_base / G + 1)) : x.len;
+    const int blk_lo = a.window > 0 ? max(0, p0 + (row_base + nrow - 1) / G - a.window + 1) : 0;
+    const int tile0 = b_lo / kPromptKeys, tiles = max(0, (b_hi + kPromptKeys - 1) / kPromptKeys - tile0);
+    const int parts = max(1, min(splits, tiles));   // with at least one tile each
+    if (split >= parts) return;
+    const int t_begin = tile0 + (int)((int64_t)tiles * split / parts), t_end = tile0 + (int)((int64_t)tiles * (split + 1) / parts);
+
+    // ---- this lane's row
+    const int wr0 = row_base + 32 * w, wrows = max(0, min(32, row_base + nrow - wr0));   // the wave's rows
+    const int r = wr0 + min(n, max(wrows - 1, 0)), tok = min(r / G, x.nq - 1), head = kvh * G + r % G;
+    const int at = p0 + tok;
+    const int hi = a.causal ? min(x.len, at + 1) : x.len, lo = a.window > 0 ? max(0, at - a.window + 1) : 0;
+    const int all_hi = a.causal ? max(0, min(x.len, p0 + wr0 / G + 1)) : x.len;
+    const int all_lo = a.window > 0 ? max(0, p0 + (wr0 + max(wrows, 1) - 1) / G - a.window + 1) : 0;
+    const int any_hi = a.causal ? max(0, min(x.len, p0 + (wr0 + max(wrows, 1) - 1) / G + 1)) : x.len;
+    const int any_lo = a.window > 0 ? max(0, p0 + wr0 / G - a.window + 1) : 0;
+    u32x4 qf[KK];
+    {
+        const uint16_t* qp = (const uint16_t*)q + (x.row0 + tok) * ldq + (int64_t)head * HD + 8 * h;
+#pragma unroll
+        for (int kk = 0; kk < KK; kk++) {
+            if (q_vec) qf[kk] = *(const u32x4*)(qp + 16 * kk);
+            else
+#pragma unroll
+                for (int i = 0; i < 4; i++) qf[kk][i] = qp[16 * kk + 2 * i] | (uint32_t)qp[16 * kk + 2 * i + 1] << 16;
+#pragma unroll
+            for (int i = 0; i < 4; i++) qf[kk][i] ^= q_sign;
+        }
+    }
+
+    // ---- staging: wave w brings the tile's keys 16 w .. 16 w + 15; page ids of 64 tiles at a time, one a lane
+    const int* tab = c.table + (int64_t)seq * c.max_pages;
+    int id = -1;
+    auto ids = [&](int t) {
+        const int64_t key = ((int64_t)t + lane) * kPromptKeys + 16 * w;
+        id = key < x.len ? tab[key >> c.page_shift] : -1;
+    };
+    Slice<HD, CT> st;   // 4-bit pages: the next tile's codes
+    bool st_ok = false;
+    auto fetch = [&](int t, int buf) {
+        if (((t - t_begin) & 63) == 0) ids(t);
+        const int d = __builtin_amdgcn_readlane(id, (t - t_begin) & 63);
+        st_ok = (unsigned)d < (unsigned)c.n_pages;
+        if (lane == 0) s_ok[buf][w] = st_ok;
+        if (!st_ok) return;
+        const int64_t b = ((int64_t)d * c.nkv + kvh) * c.block_bytes;
+        const int t0 = (t * kPromptKeys + 16 * w) & ((1 << c.page_shift) - 1);
+        if constexpr (CT == T_MXFP4) {
+            load_k<HD, CT>(st, 0, block_rsrc(c.k + b, c.block_bytes), t0, codes, lane & 15, lane >> 4);
+            load_v<HD, CT>(st, 0, block_rsrc(c.v + b, c.block_bytes), t0, codes, lane & 15, lane >> 4);
+        } else {
+            constexpr int RPI = 64 / CPR > 0 ? 64 / CPR : 1;   // rows of one 1 KB transfer
+#pragma unroll
+            for (int i = 0; i < 16 / RPI; i++) {
+                const int row = 16 * w + i * RPI + lane / CPR, pos = lane % CPR;
+                const uint32_t src = (t0 + i * RPI + lane / CPR) * ROW;
+                const uint32_t dst = buf * TILE + (16 * w + i * RPI) * ROW;
+                dma_lds16(c.k + b + src + 16 * (pos ^ k_swz<HD>(row)), (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)ldsK + dst);
+                dma_lds16(c.v + b + src + 16 * (pos ^ v_swz<HD>(row)), (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)ldsV + dst);
+            }
+        }
+    };
+    auto store = [&](int buf) {   // 4-bit pages: widened into the image that the 16-bit ones have
+        if constexpr (CT == T_MXFP4) {
+            if (!st_ok) return;
+            constexpr int ND = HD / 16;
+            const int m = lane & 15, kg = lane >> 4;
+            const uint32_t nan_k = nan_scale(st.ks[0][0]) | (HD == 256 ? nan_scale(st.ks[0][HD == 256 ? 1 : 0]) : 0u);
+#pragma unroll
+            for (int kk = 0; kk < HD / 32; kk++) {
+                const float f = __uint_as_float(((st.ks[0][kk / 4] >> (8 * (kk % 4))) & 255) << 23);
+                const uint32_t wd = st.k[0][kk];
+                u32x4 kf = {fp4_pair<QT>(wd, f, 0), fp4_pair<QT>(wd, f, 1), fp4_pair<QT>(wd, f, 2), fp4_pair<QT>(wd, f, 3)};
+                if (nan_k) kf = u32x4{0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu};   // its scores are no numbers
+                const int row = 16 * w + m, ch = kk * 4 + kg;
+                *(u32x4*)(ldsK + buf * TILE + row * ROW + 16 * (ch ^ k_swz<HD>(row))) = kf;
+            }
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const uint32_t sb = (st.vs[0] >> (8 * j)) & 255;
+                const float f = __uint_as_float(sb << 23);
+                const int row = 16 * w + 4 * kg + j;
+                uint32_t d[ND / 2];
+#pragma unroll
+                for (int b = 0; b < ND / 2; b++) {
+                    const int i = j * (ND / 2) + b;
+                    d[b] = fp4_pair<QT>(st.v[0][i / 4], f, i % 4);
+                    if (sb == 255) d[b] = 0x7fff7fffu;
+                }
+                uint8_t* dst = ldsV + buf * TILE + row * ROW;
+                if constexpr (ND == 4) {
+                    *(u32x2*)(dst + 16 * ((m / 2) ^ v_swz<HD>(row)) + 8 * (m & 1)) = u32x2{d[0], d[1]};
+                } else {
+#pragma unroll
+                    for (int p = 0; p < ND / 8; p++)
+                        *(u32x4*)(dst + 16 * ((m * (ND / 8) + p) ^ v_swz<HD>(row))) =
+                            u32x4{d[4 * p], d[4 * p + 1], d[4 * p + 2], d[4 * p + 3]};
+                }
+            }
+        }
+    };
+
+    f32x16 acc[DT];
+#pragma unroll
+    for (int i = 0; i < DT; i++)
+#pragma unroll
+        for (int j = 0; j < 16; j++) acc[i][j] = 0.f;
+    float m = kNone, l = 0.f;
+
+    // Vᵀ operand: dims 32 dt + n, key slots (h, j) = keys 32 u + 16 s + 8 (j / 4) + 4 h + j % 4
+    auto read_v = [&](int buf, int u, int s, int dt) {
+        const int g16 = (n >> 4), qr = (n & 15) >> 2, pp = n & 3;
+        s16x4 rr[2];
+#pragma unroll
+        for (int jj = 0; jj < 2; jj++) {
+            const int row = 32 * u + 16 * s + 8 * jj + 4 * h + qr, ch = 4 * dt + 2 * g16 + (pp >> 1);
+            rr[jj] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (__attribute__((address_space(3))) s16x4*)(__attribute__((address_space(3))) uint8_t*)(
+                    ldsV + buf * TILE + row * ROW + 16 * (ch ^ v_swz<HD>(row)) + 8 * (pp & 1)));
+        }
+        const u32x2 a0 = __builtin_bit_cast(u32x2, rr[0]), a1 = __builtin_bit_cast(u32x2, rr[1]);
+        return __builtin_shufflevector(a0, a1, 0, 1, 2, 3);
+    };
+
+    if (t_begin < t_end) fetch(t_begin, 0);
+    if constexpr (CT == T_MXFP4)
+        if (t_begin < t_end) store(0);
+    for (int t = t_begin; t < t_end; t++) {
+        const int buf = (t - t_begin) & 1;
+        if constexpr (CT != T_MXFP4) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();   // tile t is there, and nobody reads the other buffer any more
+        if (t + 1 < t_end) fetch(t + 1, buf ^ 1);
+        const int key = t * kPromptKeys;
+        int have = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) have |= (s_ok[buf][i] ? 1 : 0) << i;
+        have = uniform(have);
+        // 0 · V is no zero where V is no number.  In tiles that not every row of the workgroup sees whole: V that no row may
+        // use (behind the last key, no page) becomes zero, and keys of whose V any is no number (`odd`) are added apart
+        uint64_t odd = 0;
+        const int zrow = threadIdx.x >> 2;   // a quarter of a row of V for each thread
+        u32x4* const zp = (u32x4*)(ldsV + buf * TILE + zrow * ROW + (threadIdx.x & 3) * (ROW / 4));
+        if (have != 15 || key < blk_lo || key + kPromptKeys > blk_hi) {   // the same for the whole workgroup
+            const bool real = (have >> (zrow >> 4) & 1) && key + zrow < x.len;
+            constexpr uint32_t e = QT == T_F16 ? 0x7c007c00u : 0x7f807f80u;
+            u16x2 top = {0, 0};
+#pragma unroll
+            for (int i = 0; i < ROW / 64; i++) {
+                if (!real) zp[i] = u32x4{0, 0, 0, 0};
+                else {
+                    const u32x4 d = zp[i];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, d[j] & e));
+                }
+            }
+            const uint64_t bad = __ballot(top[0] == (e & 0xffffu) || top[1] == (e & 0xffffu));
+            if (lane == 0) s_odd[w] = bad;
+            __syncthreads();
+            const uint64_t some = s_odd[0] | s_odd[1] | s_odd[2] | s_odd[3];
+            if (__builtin_expect(uniform((int)(some | some >> 32)) != 0, 0))
+                for (int i = 0; i < 64; i++)
+                    if (s_odd[i >> 4] >> (4 * (i & 15)) & 15) odd |= 1ull << i;
+        }
+        const bool active = wrows > 0 && key < any_hi && key + kPromptKeys > any_lo;
+        u32x4 pf[2][2] = {};
+        uint32_t see = ~0u;   // bit 16 u + i: score i of half u
+        if (active) {
+            const bool whole = have == 15 && key >= all_lo && key + kPromptKeys <= all_hi;
+            f32x16 sv[2];
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+#pragma unroll
+                for (int j = 0; j < 16; j++) sv[u][j] = 0.f;
+#pragma unroll
+                for (int kk = 0; kk < KK; kk++) {
+                    const int row = 32 * u + n, ch = 2 * kk + h;
+                    const u32x4 kf = *(const u32x4*)(ldsK + buf * TILE + row * ROW + 16 * (ch ^ k_swz<HD>(row)));
+                    sv[u] = mfma32<QT>(kf, qf[kk], sv[u]);
+                }
+            }
+            if (!whole) {
+                const int k4 = key + 4 * anew(h);
+                see = 0;
+#pragma unroll
+                for (int u = 0; u < 2; u++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        const int kj = k4 + 32 * u + 8 * (i / 4) + i % 4;
+                        if ((have >> (2 * u + i / 8) & 1) && kj >= lo && kj < hi) see |= 1u << (16 * u + i);
+                        else sv[u][i] = -INFINITY;
+                    }
+            }
+            float mx = sv[0][0];
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) mx = fmaxf(mx, sv[u][i]);
+            mx *= sc;
+            if (__any(mx > m + kSlack)) {
+                mx = fmaxf(mx, __shfl_xor(mx, 32));
+                const float mn = fmaxf(m, mx), al = __builtin_amdgcn_exp2f(m - mn);
+                m = mn;
+                l *= al;
+#pragma unroll
+                for (int i = 0; i < DT; i++) acc[i] *= al;
+            }
+            const float mk = kUp - m;
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                float ls = 0.f;
+#pragma unroll
+                for (int i = 0; i < 16; i += 2) {
+                    const float e0 = __builtin_amdgcn_exp2f(fmaf(sv[u][i], sc, mk));
+                    const float e1 = __builtin_amdgcn_exp2f(fmaf(sv[u][i + 1], sc, mk));
+                    ls += e0 + e1;
+                    pf[u][i / 8][(i % 8) / 2] = pack2<QT>(e0, e1);
+                }
+                l += ls;
+            }
+        }
+        if (__builtin_expect(odd != 0, 0)) {
+            for (uint64_t todo = active ? odd : 0; todo; todo &= todo - 1) {
+                const int ki = __builtin_ctzll(todo), kk = ki & 31, own = kk >> 2 & 1;   // the lane half that has its weight
+                const int idx = (ki >> 5) * 16 + (kk >> 3) * 4 + (kk & 3);
+                uint32_t two = 0;
+#pragma unroll
+                for (int j = 0; j < 16; j++)
+                    if (idx >> 1 == j) two = pf[j / 8][(j % 8) / 4][j % 4];
+                const uint16_t pb = (uint16_t)(idx & 1 ? two >> 16 : two);
+                float pw = QT == T_F16 ? (float)__builtin_bit_cast(_Float16, pb) : (float)__builtin_bit_cast(__bf16, pb);
+                int sees = see >> idx & 1;
+                const float pw2 = __shfl_xor(pw, 32);
+                const int sees2 = __shfl_xor(sees, 32);
+                if (h != own) pw = pw2, sees = sees2;
+#pragma unroll
+                for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+                    for (int g = 0; g < 4; g++) {
+                        const int ch = 4 * dt + g;
+                        const uint16_t* vp = (const uint16_t*)(ldsV + buf * TILE + ki * ROW + 16 * (ch ^ v_swz<HD>(ki)) + 8 * h);
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const float vv = QT == T_F16 ? (float)__builtin_bit_cast(_Float16, vp[i]) : (float)__builtin_bit_cast(__bf16, vp[i]);
+                            if (sees) acc[dt][4 * g + i] = fmaf(pw, vv, acc[dt][4 * g + i]);
+                        }
+                    }
+            }
+            __syncthreads();
+            if (odd >> zrow & 1)
+#pragma unroll
+                for (int i = 0; i < ROW / 64; i++) zp[i] = u32x4{0, 0, 0, 0};
+            __syncthreads();
+        }
+        if (active) {
+#pragma unroll
+            for (int us = 0; us < 4; us++)
+#pragma unroll
+                for (int dt = 0; dt < DT; dt++)
+                    acc[dt] = mfma32<QT>(read_v(buf, us >> 1, us & 1, dt), pf[us >> 1][us & 1], acc[dt]);
+        }
+        if constexpr (CT == T_MXFP4)
+            if (t + 1 < t_end) store(buf ^ 1);
+    }
+    l += __shfl_xor(l, 32);
+
+    // ---- out, or joined with the item's other parts
+    bool write = true;
+    if (parts > 1) {
+        const int item_slot = item * splits;
+        float* mine = part + (int64_t)(item_slot + split) * kSlot;
+        const uint32_t off = ((w * DT * 4) * 64 + lane) * 16;
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+            for (int g = 0; g < 4; g++)
+                wt_st128(mine, off + (dt * 4 + g) * 1024,
+                         __builtin_bit_cast(wt_v4i, f32x4{acc[dt][4 * g], acc[dt][4 * g + 1], acc[dt][4 * g + 2], acc[dt][4 * g + 3]}));
+        if (h == 0) {
+            wt_stf(mine, (kRowBlock * HD + 32 * w + n) * 4, m);
+            wt_stf(mine, (kRowBlock * (HD + 1) + 32 * w + n) * 4, l);
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // written through before the arrival is counted
+        __syncthreads();
+        if (threadIdx.x == 0)
+            s_last = __hip_atomic_fetch_add(&cnt[item], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)parts - 1;
+        __syncthreads();
+        write = s_last;
+        if (write) {
+            if (threadIdx.x == 0) __hip_atomic_store(&cnt[item], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            float M = kNone;
+            for (int pc = 0; pc < parts; pc++)
+                M = fmaxf(M, wt_ldf(part + (int64_t)(item_slot + pc) * kSlot, (kRowBlock * HD + 32 * w + n) * 4));
+            l = 0.f;
+#pragma unroll
+            for (int i = 0; i < DT; i++)
+#pragma unroll
+                for (int j = 0; j < 16; j++) acc[i][j] = 0.f;
+            for (int pc = 0; pc < parts; pc++) {
+                const float* src = part + (int64_t)(item_slot + pc) * kSlot;
+                const float f = __builtin_amdgcn_exp2f(wt_ldf(src, (kRowBlock * HD + 32 * w + n) * 4) - M);
+                l = fmaf(wt_ldf(src, (kRowBlock * (HD + 1) + 32 * w + n) * 4), f, l);
+#pragma unroll
+                for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+                    for (int g = 0; g < 4; g++) {
+                        const float4 v4 = wt_ldf4(src, off + (dt * 4 + g) * 1024);
+                        acc[dt][4 * g] = fmaf(v4.x, f, acc[dt][4 * g]);
+                        acc[dt][4 * g + 1] = fmaf(v4.y, f, acc[dt][4 * g + 1]);
+                        acc[dt][4 * g + 2] = fmaf(v4.z, f, acc[dt][4 * g + 2]);
+                        acc[dt][4 * g + 3] = fmaf(v4.w, f, acc[dt][4 * g + 3]);
+                    }
+            }
+        }
+    }
+    if (write && n < wrows) {
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const int64_t at_o = (x.row0 + tok) * ldo + (int64_t)head * HD + 4 * h;
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                f32x4 v4 = {acc[dt][4 * g], acc[dt][4 * g + 1], acc[dt][4 * g + 2], acc[dt][4 * g + 3]};
+                v4 *= inv;
+                store_out<QT>(o, a.o_type, at_o + 32 * dt + 8 * g, v4, o_vec);
+            }
+    }
+}
+
 }  // namespace
 
+// which kernel: prompts fill 32-row matrix tiles, single tokens and short verify passes do not
+static bool is_prompt(const KvPages& c, const AttnArgs& a) { return (int64_t)a.max_q * (a.nh / c.nkv) > 32; }
+constexpr int kPromptSlots = 512;   // parts at most where items are split
+
 size_t paged_attention_ws(const KvPages& c, const AttnArgs& a) {
-    return (size_t)kSplitWgs * 4 + (size_t)kSplitWgs * 2 * (16 * c.hd + 32) * 4;
+    const size_t few = (size_t)kSplitWgs * 4 + (size_t)kSplitWgs * 2 * (16 * c.hd + 32) * 4;
+    const size_t many = (size_t)kSplitWgs * 4 + (size_t)kPromptSlots * kRowBlock * (c.hd + 2) * 4;
+    return is_prompt(c, a) ? many : few;
 }
 
 template <int HD, int CT, int QT>
 static void launch(const KvPages& c, const AttnArgs& a, const void* q, int64_t ldq, const int* q_start,
                    const int* kv_len, int rows, void* o, int64_t ldo, void* ws, hipStream_t s) {
-    const int G = a.nh / c.nkv, min_tiles = 1;
-    const int64_t items = ((int64_t)rows * G / 16 + c.n_seq) * c.nkv;   // at most
-    const int64_t tiles = items * std::max<int64_t>(1, cdiv64(a.max_kv, kTileKeys));
-    const int grid = (int)std::min<int64_t>(256 * wgs_per_cu(HD, CT), std::max<int64_t>(1, cdiv64(tiles, min_tiles)));
+    const int G = a.nh / c.nkv;
     const int q_vec = ldq % 8 == 0 && ((uintptr_t)q & 15) == 0;
     const int o_vec = ldo % 4 == 0 && ((uintptr_t)o & 15) == 0;
-    k_paged_attn<HD, CT, QT><<<grid, 256, 0, s>>>(c, a, q, ldq, q_start, kv_len, rows, o, ldo,
-                                                  (float*)((char*)ws + kSplitWgs * 4), (unsigned*)ws, min_tiles, q_vec,
+    unsigned* cnt = (unsigned*)ws;
+    float* part = (float*)((char*)ws + kSplitWgs * 4);
+    if (is_prompt(c, a)) {
+        const int64_t items = ((int64_t)rows * G / kRowBlock + c.n_seq) * c.nkv;   // at most
+        QASR_CHECK(items < 1 << 23, QASR_E_CAPACITY, "paged_attention: too many rows for one call");
+        const int splits = (int)std::max<int64_t>(1, kPromptSlots / items);
+        const size_t lds = 4 * kPromptKeys * HD * 2;
+        if (lds > 65536) {
+            static const bool set = [&] {
+                QASR_HIP(hipFuncSetAttribute((const void*)k_paged_prompt<HD, CT, QT>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+                return true;
+            }();
+            (void)set;
+        }
+        k_paged_prompt<HD, CT, QT><<<(unsigned)(items * splits), 256, lds, s>>>(c, a, q, ldq, q_start, kv_len, rows, o, ldo,
+                                                                               part, cnt, splits, q_vec, o_vec);
+        return;
+    }
+    const int min_tiles = 1;
+    const int64_t items = ((int64_t)rows * G / 16 + c.n_seq) * c.nkv;   // at most
+    QASR_CHECK(items * cdiv64(((int64_t)c.max_pages << c.page_shift) + 1, kTileKeys) < 1 << 30, QASR_E_CAPACITY,
+               "paged_attention: too many rows for the max_q that they were announced with");
+    const int64_t tiles = items * std::max<int64_t>(1, cdiv64(a.max_kv, kTileKeys));
+    const int grid = (int)std::min<int64_t>(256 * wgs_per_cu(HD, CT), std::max<int64_t>(1, cdiv64(tiles, min_tiles)));
+    k_paged_attn<HD, CT, QT><<<grid, 256, 0, s>>>(c, a, q, ldq, q_start, kv_len, rows, o, ldo, part, cnt, min_tiles, q_vec,
                                                   o_vec);
 }
 

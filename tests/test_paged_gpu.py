@@ -428,18 +428,20 @@ def test_attention_nothing_outside_the_keys(torch_dev, kv, qt, nq):
         o = attend(c, q, qs, kl, 4, True, 0, 0.09, max_q=hints[0], max_kv=hints[1])
         check_attend(c, q, o, qs, kl, 4, True, 0, 0.09, qt, qt, values=clean)
         assert (num(o)[rows:] == 9).all()
-    # NaN in the last key: only the rows that see it take it
+    # NaN in the last key: only the rows that see it take it (in either way of splitting the work)
+    before = [num(attend(c, q, qs, kl, 4, True, 0, 0.09, max_q=m)) for m in (1, 1000)]
     ids, t = c.table_h[2, 199 // 16], 199 % 16
     for j, p in enumerate(c.pools):
         if kv == "mxfp4":
             p[int(ids), :, dev(ref.fp4_offsets(128, 16, j == 1)[1][t])] = 255
         else:
             p[int(ids), :, t] = float("inf") if j else float("nan")
-    o2 = num(attend(c, q, qs, kl, 4, True, 0, 0.09))
     last = int(qs[3]) - 1
-    assert np.isnan(o2[last]).all()
     same = np.arange(rows) != last
-    assert np.array_equal(o2[:rows][same], num(o)[:rows][same])
+    for m, was in zip((1, 1000), before):
+        o2 = num(attend(c, q, qs, kl, 4, True, 0, 0.09, max_q=m))
+        assert np.isnan(o2[last]).all()
+        assert np.array_equal(o2[:rows][same], was[:rows][same])
 
 
 @pytest.mark.parametrize("kv,qt", LAYOUTS)
