@@ -24,6 +24,7 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
+constexpr int kPieces = 32;      // parts of one item at most
 constexpr int kTileKeys = 128;   // keys of one workgroup step: 32 for each of its 4 waves
 constexpr int kSplitWgs = 1024;  // workgroups at most (what the scratch is sized for)
 // workgroups that a CU holds by their registers
@@ -79,15 +80,29 @@ __device__ __forceinline__ uint32_t lo16(uint32_t a, uint32_t b) { return __buil
 __device__ __forceinline__ uint32_t hi16(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
-// inclusive prefix sum over the wave
+// inclusive prefix sum over the wave, and its maximum (of values >= 0), on DPP: rows of 16 by shifts, then each row's last
+// lane to the rows behind it
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_or_0(int v) {
+    return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
+}
 __device__ __forceinline__ int wave_scan(int v) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int u = __shfl_up(v, o);
-        if (lane >= o) v += u;
-    }
+    v += dpp_or_0<0x111, 0xf>(v);
+    v += dpp_or_0<0x112, 0xf>(v);
+    v += dpp_or_0<0x114, 0xf>(v);
+    v += dpp_or_0<0x118, 0xf>(v);
+    v += dpp_or_0<0x142, 0xa>(v);
+    v += dpp_or_0<0x143, 0xc>(v);
     return v;
+}
+__device__ __forceinline__ int wave_top(int v) {
+    v = max(v, dpp_or_0<0x111, 0xf>(v));
+    v = max(v, dpp_or_0<0x112, 0xf>(v));
+    v = max(v, dpp_or_0<0x114, 0xf>(v));
+    v = max(v, dpp_or_0<0x118, 0xf>(v));
+    v = max(v, dpp_or_0<0x142, 0xa>(v));
+    v = max(v, dpp_or_0<0x143, 0xc>(v));
+    return __builtin_amdgcn_readlane(v, 63);
 }
 
 // what one sequence asks for (per lane while scanning, uniform afterwards)
@@ -285,7 +300,7 @@ template <int HD, int CT, int QT>
 __global__ __launch_bounds__(256, wgs_per_cu(HD, CT)) void k_paged_attn(KvPages c, AttnArgs a, const void* __restrict__ q, int64_t ldq,
                                                        const int* __restrict__ q_start, const int* __restrict__ kv_len,
                                                        int rows, void* __restrict__ o, int64_t ldo, float* part,
-                                                       unsigned* cnt, int min_tiles, int q_vec, int o_vec) {
+                                                       unsigned* cnt, int q_vec, int o_vec) {
     constexpr int ND = HD / 16, KK = HD / 32, LANES = 64;
     constexpr int kSlot = 16 * HD + 32;   // floats of a slot: Oᵀ as [wave][lane >> 4][row][ND], then m and l of 16 rows
     __shared__ float s_acc[4][ND * 4][LANES];
@@ -303,6 +318,7 @@ __global__ __launch_bounds__(256, wgs_per_cu(HD, CT)) void k_paged_attn(KvPages 
         return max(1, (x.len + kTileKeys - 1) / kTileKeys - x.lo / kTileKeys);
     };
     auto items_of = [&](const SeqWork& x) { return ((x.nq * G + 15) >> 4) * c.nkv; };
+    int longest = 0;                        // item, in tiles
     int chunk = 0, before = 0, total = 0;   // first sequence held in the lanes, tiles before it, all tiles
     SeqWork my{};
     int scan = 0;   // tiles up to and with this lane's sequence, from `chunk` on
@@ -315,8 +331,10 @@ __global__ __launch_bounds__(256, wgs_per_cu(HD, CT)) void k_paged_attn(KvPages 
     for (int s0 = 0; s0 < c.n_seq; s0 += LANES) {
         hold(s0);
         total += __builtin_amdgcn_readlane(scan, 63);
+        longest = max(longest, wave_top(my.nq > 0 ? tiles_of(my) : 0));
     }
-    const int per = max(min_tiles, (total + (int)gridDim.x - 1) / (int)gridDim.x);
+    // a long item in at most kPieces parts: their arrivals are counted one after the other, 40 to 80 ns each
+    const int per = max((total + (int)gridDim.x - 1) / (int)gridDim.x, (longest + kPieces - 1) / kPieces);
     int t = blockIdx.x * per;
     const int t_end = min(total, t + per);
     if (t >= t_end) return;
@@ -1093,13 +1111,12 @@ static void launch(const KvPages& c, const AttnArgs& a, const void* q, int64_t l
                                                                                part, cnt, splits, q_vec, o_vec);
         return;
     }
-    const int min_tiles = 1;
     const int64_t items = ((int64_t)rows * G / 16 + c.n_seq) * c.nkv;   // at most
     QASR_CHECK(items * cdiv64(((int64_t)c.max_pages << c.page_shift) + 1, kTileKeys) < 1 << 30, QASR_E_CAPACITY,
                "paged_attention: too many rows for the max_q that they were announced with");
     const int64_t tiles = items * std::max<int64_t>(1, cdiv64(a.max_kv, kTileKeys));
-    const int grid = (int)std::min<int64_t>(256 * wgs_per_cu(HD, CT), std::max<int64_t>(1, cdiv64(tiles, min_tiles)));
-    k_paged_attn<HD, CT, QT><<<grid, 256, 0, s>>>(c, a, q, ldq, q_start, kv_len, rows, o, ldo, part, cnt, min_tiles, q_vec,
+    const int grid = (int)std::min<int64_t>(256 * wgs_per_cu(HD, CT), tiles);
+    k_paged_attn<HD, CT, QT><<<grid, 256, 0, s>>>(c, a, q, ldq, q_start, kv_len, rows, o, ldo, part, cnt, q_vec,
                                                   o_vec);
 }
 
