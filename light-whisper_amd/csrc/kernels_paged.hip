@@ -1,4 +1,7 @@
 // Rotary positions, their table, and moving rows into and out of paged K/V caches (include/qasr.h, "paged K/V cache").
+#include <algorithm>
+#include <type_traits>
+
 #include "paged_dev.h"
 
 namespace qasr {
@@ -78,18 +81,178 @@ __device__ void head_to_lds(const void* x, int64_t off, int hd, const RopeArgs& 
     lds_sync_wave();
 }
 
+// ---- the fast form: a thread takes 16 dims of a head, as two runs of 8 with 16-byte accesses: dims 8 u and rot/2 + 8 u in
+// the half layout (each pair in one thread), 16 u and 16 u + 8 in the interleaved one and behind the rotated dims.  The
+// head's hd / 16 threads are neighbours, so a run of lanes reads a run of bytes and the norm's sum is a few xor-shuffles.
+// A thread takes up to four heads of its row with one read of the table.  Bound by memory.
+constexpr int kHeadsPer = 4;
+
+template <int T>
+__device__ __forceinline__ void load8(const void* p, int64_t at, float (&v)[8]) {
+    if constexpr (T == T_F32) {
+        const float4 a = *(const float4*)((const float*)p + at), b = *(const float4*)((const float*)p + at + 4);
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    } else if constexpr (T == T_F16) {
+        const f16x8 a = *(const f16x8*)((const uint16_t*)p + at);
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = (float)a[i];
+    } else {
+        const bf16x8 a = *(const bf16x8*)((const uint16_t*)p + at);
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = (float)a[i];
+    }
+}
+template <int T>
+__device__ __forceinline__ void store8(void* p, int64_t at, const float (&v)[8]) {
+    if constexpr (T == T_F32) {
+        *(float4*)((float*)p + at) = make_float4(v[0], v[1], v[2], v[3]);
+        *(float4*)((float*)p + at + 4) = make_float4(v[4], v[5], v[6], v[7]);
+    } else if constexpr (T == T_F16) {
+        f16x8 a;
+#pragma unroll
+        for (int i = 0; i < 8; i++) a[i] = (_Float16)v[i];
+        *(f16x8*)((uint16_t*)p + at) = a;
+    } else {
+        bf16x8 a;
+#pragma unroll
+        for (int i = 0; i < 8; i++) a[i] = (__bf16)v[i];
+        *(bf16x8*)((uint16_t*)p + at) = a;
+    }
+}
+// whether rows can be read and written 16 bytes at a time
+static bool rows16(const Rows& r) { return ((uintptr_t)r.p & 15) == 0 && r.ld * elem_bytes(r.type) % 16 == 0; }
+static bool units_ok(int hd, const RopeArgs& r) {
+    return hd % 16 == 0 && (!r.cs || (r.rot % 16 == 0 && ((uintptr_t)r.cs & 15) == 0)) && ((uintptr_t)r.norm_w & 15) == 0;
+}
+
+// a thread's place in a head, the same for all rows
+struct Unit {
+    int a, b;      // its two runs' first dims
+    bool turn;     // they rotate
+};
+__device__ __forceinline__ Unit unit_of(int u, const RopeArgs& r) {
+    const int n = r.cs ? r.rot / 16 : 0;
+    if (u < n && !r.interleaved) return Unit{8 * u, r.rot / 2 + 8 * u, true};
+    return Unit{16 * u, 16 * u + 8, u < n};
+}
+// norm and rotation of the 16 dims; cs: the row's table entries of the unit (8 of cos, sin), w: its norm weights.
+// `lanes`: threads of a head rounded up to a power of two; those without dims hold zeros
+template <typename A>
+__device__ __forceinline__ void turn16(A (&x)[2][8], const Unit& un, const RopeArgs& r, int hd, int lanes,
+                                       const float (&cs)[16], const float (&w)[2][8]) {
+    if (r.norm_w) {
+        A ss = 0;
+#pragma unroll
+        for (int i = 0; i < 8; i++) ss += x[0][i] * x[0][i] + x[1][i] * x[1][i];
+        for (int o = lanes >> 1; o > 0; o >>= 1) ss += shfl_xor_t<A>(ss, o);
+        A inv;
+        if constexpr (sizeof(A) == 8) inv = 1.0 / sqrt(ss / (double)hd + (double)r.eps);
+        else inv = rsqrtf(ss / (float)hd + r.eps);
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            x[0][i] = x[0][i] * inv * (A)w[0][i];
+            x[1][i] = x[1][i] * inv * (A)w[1][i];
+        }
+    }
+    if (!un.turn) return;
+    if (r.interleaved) {
+#pragma unroll
+        for (int k = 0; k < 2; k++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const A c = cs[8 * k + 2 * i], s = cs[8 * k + 2 * i + 1], u = x[k][2 * i], v = x[k][2 * i + 1];
+                x[k][2 * i] = u * c - v * s;
+                x[k][2 * i + 1] = v * c + u * s;
+            }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const A c = cs[2 * i], s = cs[2 * i + 1], u = x[0][i], v = x[1][i];
+            x[0][i] = u * c - v * s;
+            x[1][i] = v * c + u * s;
+        }
+    }
+}
+__device__ __forceinline__ void load_unit_consts(const Unit& un, const RopeArgs& r, int p, int u, float (&cs)[16],
+                                                 float (&w)[2][8]) {
+    if (un.turn) {
+        const float4* t = (const float4*)(r.cs + ((int64_t)p * (r.rot / 2) + 8 * u) * 2);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float4 v = t[i];
+            cs[4 * i] = v.x, cs[4 * i + 1] = v.y, cs[4 * i + 2] = v.z, cs[4 * i + 3] = v.w;
+        }
+    }
+    if (r.norm_w) {
+        load8<T_F32>(r.norm_w, un.a, w[0]);
+        load8<T_F32>(r.norm_w, un.b, w[1]);
+    }
+}
+
+// grid: (row, group of HP heads) items, 256 / lanes of them a workgroup
+template <int XT, int YT, int HP>
+__global__ __launch_bounds__(256) void k_rope_units(const void* x, int64_t ldx, const int* __restrict__ pos, int rows,
+                                                    int heads, int hd, int lanes_log2, RopeArgs r, void* y, int64_t ldy) {
+    const int lanes = 1 << lanes_log2, u = threadIdx.x & (lanes - 1), groups = (heads + HP - 1) / HP;
+    const bool mine = u < hd / 16;
+    const Unit un = unit_of(u, r);
+    const int64_t items = (int64_t)rows * groups, step = (int64_t)gridDim.x * (256 >> lanes_log2);
+    for (int64_t it = (int64_t)blockIdx.x * (256 >> lanes_log2) + (threadIdx.x >> lanes_log2); it < items; it += step) {
+        const int row = (int)(it / groups), h0 = (int)(it % groups) * HP;
+        const int p = r.cs ? pos[row] : 0;
+        if (r.cs && (unsigned)p >= (unsigned)r.n_pos) continue;   // the whole group of lanes
+        float cs[16], w[2][8], v[HP][2][8];
+        if (mine) {
+            load_unit_consts(un, r, p, u, cs, w);
+#pragma unroll
+            for (int k = 0; k < HP; k++)
+                if (h0 + k < heads) {
+                    const int64_t at = row * ldx + (int64_t)(h0 + k) * hd;
+                    load8<XT>(x, at + un.a, v[k][0]);
+                    load8<XT>(x, at + un.b, v[k][1]);
+                }
+        }
+#pragma unroll
+        for (int k = 0; k < HP; k++) {
+            if (h0 + k >= heads) break;
+            if (!mine)
+#pragma unroll
+                for (int i = 0; i < 8; i++) v[k][0][i] = v[k][1][i] = 0.f;
+            turn16<float>(v[k], un, r, hd, lanes, cs, w);
+            if (mine) {
+                const int64_t at = row * ldy + (int64_t)(h0 + k) * hd;
+                store8<YT>(y, at + un.a, v[k][0]);
+                store8<YT>(y, at + un.b, v[k][1]);
+            }
+        }
+    }
+}
+static int log2_up(int n) {
+    int l = 0;
+    while (1 << l < n) l++;
+    return l;
+}
+static unsigned unit_grid(int64_t items, int lanes_log2) {   // enough workgroups to fill the chip several times over
+    return (unsigned)std::min<int64_t>(cdiv64(items, 256 >> lanes_log2), 256 * 32);
+}
+
+// ---- any other: a head a wave, through LDS, element by element
 constexpr int kRopeMaxHd = 1024;
 
 template <int XT, int YT>
-__global__ __launch_bounds__(64) void k_rope_any(const void* x, int64_t ldx, const int* __restrict__ pos, int heads,
+__global__ __launch_bounds__(64) void k_rope_any(const void* x, int64_t ldx, const int* __restrict__ pos, int rows, int heads,
                                                  int hd, RopeArgs r, void* y, int64_t ldy) {
     __shared__ float buf[kRopeMaxHd];
-    const int row = blockIdx.x / heads, head = blockIdx.x % heads, lane = threadIdx.x;
-    const int p = r.cs ? pos[row] : 0;
-    if (r.cs && (unsigned)p >= (unsigned)r.n_pos) return;
-    head_to_lds<XT, float>(x, row * ldx + (int64_t)head * hd, hd, r, p, lane, buf);
-    auto* o = (typename Elem<YT>::type*)y + row * ldy + (int64_t)head * hd;
-    for (int d = lane; d < hd; d += 64) o[d] = (typename Elem<YT>::type)buf[d];
+    const int lane = threadIdx.x;
+    for (int64_t it = blockIdx.x; it < (int64_t)rows * heads; it += gridDim.x) {
+        const int row = (int)(it / heads), head = (int)(it % heads);
+        const int p = r.cs ? pos[row] : 0;
+        if (r.cs && (unsigned)p >= (unsigned)r.n_pos) continue;
+        head_to_lds<XT, float>(x, row * ldx + (int64_t)head * hd, hd, r, p, lane, buf);
+        auto* o = (typename Elem<YT>::type*)y + row * ldy + (int64_t)head * hd;
+        for (int d = lane; d < hd; d += 64) o[d] = (typename Elem<YT>::type)buf[d];
+        lds_sync_wave();
+    }
 }
 
 template <class F>
@@ -104,101 +267,232 @@ void rope_rows(const Rows& x, const int* pos, int rows, int heads, int hd, const
     if (rows <= 0) return;
     by_type(x.type, [&](auto xt) {
         by_type(y.type, [&](auto yt) {
-            k_rope_any<xt(), yt()><<<(unsigned)rows * heads, 64, 0, s>>>(x.p, x.ld, pos, heads, hd, r, (void*)y.p, y.ld);
+            constexpr int XT = xt(), YT = yt();
+            if (units_ok(hd, r) && rows16(x) && rows16(y)) {
+                const int ll = log2_up(hd / 16);
+                // few rows: a head a thread group, so that more of the chip works on them; many: four
+                const int64_t all = (int64_t)rows * heads;
+                if (all << ll < 65536)
+                    k_rope_units<XT, YT, 1><<<unit_grid(all, ll), 256, 0, s>>>(x.p, x.ld, pos, rows, heads, hd, ll, r,
+                                                                               (void*)y.p, y.ld);
+                else
+                    k_rope_units<XT, YT, kHeadsPer><<<unit_grid((int64_t)rows * cdiv(heads, kHeadsPer), ll), 256, 0, s>>>(
+                        x.p, x.ld, pos, rows, heads, hd, ll, r, (void*)y.p, y.ld);
+            } else {
+                k_rope_any<XT, YT><<<(unsigned)std::min<int64_t>((int64_t)rows * heads, 1 << 20), 64, 0, s>>>(
+                    x.p, x.ld, pos, rows, heads, hd, r, (void*)y.p, y.ld);
+            }
         });
     });
 }
 
 // ------------------------------------------------------------------------------------------------ append / gather
-// one (row, KV head) by one wave
+// 8 codes of values that share a scale byte (255: none)
+__device__ __forceinline__ uint32_t fp4_codes8(const float (&v)[8], int scale) {
+    if (scale == 255) return 0;
+    const float f = __uint_as_float((uint32_t)scale << 23);   // v / f to the nearest code, ties to the even one, saturating
+    uint32_t d = 0;
+    d = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(d, v[0], v[1], f, 0);
+    d = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(d, v[2], v[3], f, 1);
+    d = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(d, v[4], v[5], f, 2);
+    d = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(d, v[6], v[7], f, 3);
+    return d;
+}
+__device__ __forceinline__ uint32_t top8(const float (&v)[8]) {   // the largest |v| by its bits, so that NaN counts
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+    return m;
+}
+// two runs of 8 dims (first dims a and b) of token t into an MXFP4 block; `wide`: they lie in blocks of 32 of their own,
+// which 4 neighbouring threads share, else 2 threads' 32 dims are one block
+__device__ __forceinline__ void fp4_put(uint8_t* blk, uint32_t codes, int hd, int t, bool is_v, int a, int b, bool wide,
+                                        const float (&x)[2][8]) {
+    uint32_t m0 = top8(x[0]), m1 = top8(x[1]);
+    const uint32_t both = max(m0, m1);
+    if (!wide) m0 = m1 = both;
+    m0 = max(m0, (uint32_t)__shfl_xor((int)m0, 1));
+    m1 = max(m1, (uint32_t)__shfl_xor((int)m1, 1));
+    const uint32_t n0 = max(m0, (uint32_t)__shfl_xor((int)m0, 2)), n1 = max(m1, (uint32_t)__shfl_xor((int)m1, 2));
+    if (wide) m0 = n0, m1 = n1;
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const int d = k ? b : a, sc = fp4_scale(__uint_as_float(k ? m1 : m0));
+        const uint32_t w = fp4_codes8(x[k], sc);
+        if (is_v && hd == 64) {   // 4 dims lie together
+            *(uint16_t*)(blk + fp4_v_code(hd, t, d)) = (uint16_t)w;
+            *(uint16_t*)(blk + fp4_v_code(hd, t, d + 4)) = (uint16_t)(w >> 16);
+        } else {
+            *(uint32_t*)(blk + (is_v ? fp4_v_code : fp4_k_code)(hd, t, d)) = w;
+        }
+        if (d % 32 == 0) blk[codes + (is_v ? fp4_v_scale : fp4_k_scale)(hd, t, d)] = (uint8_t)sc;
+    }
+}
+
+// a thread: 16 dims of K and of V of one KV head (as k_rope_units; hd is a power of two, so every thread has dims)
 template <int XT, int CT>
-__global__ __launch_bounds__(64) void k_kv_append(KvPages c, const void* k, const void* v, int64_t ldk, int64_t ldv,
-                                                  const int* __restrict__ seq, const int* __restrict__ pos, RopeArgs r) {
+__global__ __launch_bounds__(256) void k_kv_append_units(KvPages c, const void* k, const void* v, int64_t ldk, int64_t ldv,
+                                                         const int* __restrict__ seq, const int* __restrict__ pos, int rows,
+                                                         RopeArgs r) {
     // 4-bit pages: K in 64 bits up to the rounding to f32, so that a value next to a border between two codes gets its own
     typedef typename std::conditional<CT == T_MXFP4, double, float>::type A;
-    __shared__ A buf[256];
-    const int row = blockIdx.x / c.nkv, head = blockIdx.x % c.nkv, lane = threadIdx.x;
-    const int p = pos[row];
-    if (r.cs && (unsigned)p >= (unsigned)r.n_pos) return;
-    const int64_t at = page_block(c, seq[row], p, head);
-    if (at < 0) return;
-    const int t = p & ((1 << c.page_shift) - 1);
-    const RopeArgs none{};
-    for (int kv = 0; kv < 2; kv++) {
-        uint8_t* blk = (kv ? c.v : c.k) + at;
-        head_to_lds<XT, A>(kv ? v : k, row * (kv ? ldv : ldk) + (int64_t)head * c.hd, c.hd, kv ? none : r, p, lane, buf);
+    const int lanes = c.hd / 16, ll = 31 - __builtin_clz(lanes), u = threadIdx.x & (lanes - 1);
+    const Unit un = unit_of(u, r);
+    const int64_t items = (int64_t)rows * c.nkv, step = (int64_t)gridDim.x * (256 >> ll);
+    const uint32_t codes = (c.hd / 2) << c.page_shift;
+    for (int64_t it = (int64_t)blockIdx.x * (256 >> ll) + (threadIdx.x >> ll); it < items; it += step) {
+        const int row = (int)(it / c.nkv), head = (int)(it % c.nkv);
+        const int p = pos[row];
+        const int64_t at = r.cs && (unsigned)p >= (unsigned)r.n_pos ? -1 : page_block(c, seq[row], p, head);
+        if (at < 0) continue;   // the whole group of lanes
+        float cs[16], w[2][8], kx[2][8], vx[2][8];
+        const int64_t ka = row * ldk + (int64_t)head * c.hd, va = row * ldv + (int64_t)head * c.hd;
+        load8<XT>(k, ka + un.a, kx[0]);
+        load8<XT>(k, ka + un.b, kx[1]);
+        load8<XT>(v, va + 16 * u, vx[0]);
+        load8<XT>(v, va + 16 * u + 8, vx[1]);
+        load_unit_consts(un, r, p, u, cs, w);
+        A x[2][8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[0][i] = kx[0][i], x[1][i] = kx[1][i];
+        turn16<A>(x, un, r, c.hd, lanes, cs, w);
+#pragma unroll
+        for (int i = 0; i < 8; i++) kx[0][i] = (float)x[0][i], kx[1][i] = (float)x[1][i];
+        const int t = p & ((1 << c.page_shift) - 1);
         if constexpr (CT == T_MXFP4) {
-            const uint32_t codes = (c.hd / 2) << c.page_shift;
-            if (4 * lane < c.hd) {   // four dims of one block of 32
-                uint32_t am = 0;
-                for (int i = 0; i < 32; i++)
-                    am = max(am, __float_as_uint((float)buf[(4 * lane) / 32 * 32 + i]) & 0x7fffffffu);
-                const int sc = fp4_scale(__uint_as_float(am));
-                uint32_t w = 0;
-                for (int i = 0; i < 4; i++) w |= fp4_code((float)buf[4 * lane + i], sc) << (4 * i);
-                *(uint16_t*)(blk + (kv ? fp4_v_code : fp4_k_code)(c.hd, t, 4 * lane)) = (uint16_t)w;
-                if (lane % 8 == 0) blk[codes + (kv ? fp4_v_scale : fp4_k_scale)(c.hd, t, 4 * lane)] = (uint8_t)sc;
-            }
+            fp4_put(c.k + at, codes, c.hd, t, false, un.a, un.b, un.turn && !r.interleaved, kx);
+            fp4_put(c.v + at, codes, c.hd, t, true, 16 * u, 16 * u + 8, false, vx);
         } else {
-            typedef typename Elem<CT>::type E;
-            for (int d = lane; d < c.hd; d += 64) ((E*)blk)[t * c.hd + d] = (E)(float)buf[d];
+            store8<CT>(c.k + at, (int64_t)t * c.hd + un.a, kx[0]);
+            store8<CT>(c.k + at, (int64_t)t * c.hd + un.b, kx[1]);
+            store8<CT>(c.v + at, (int64_t)t * c.hd + 16 * u, vx[0]);
+            store8<CT>(c.v + at, (int64_t)t * c.hd + 16 * u + 8, vx[1]);
         }
-        lds_sync_wave();
     }
+}
+
+// any other alignment or rotation: one (row, KV head) by one wave, through LDS
+template <int XT, int CT>
+__global__ __launch_bounds__(64) void k_kv_append_any(KvPages c, const void* k, const void* v, int64_t ldk, int64_t ldv,
+                                                      const int* __restrict__ seq, const int* __restrict__ pos, int rows,
+                                                      RopeArgs r) {
+    typedef typename std::conditional<CT == T_MXFP4, double, float>::type A;   // as above
+    __shared__ A buf[256];
+    const int lane = threadIdx.x;
+    const RopeArgs none{};
+    for (int64_t it = blockIdx.x; it < (int64_t)rows * c.nkv; it += gridDim.x) {
+        const int row = (int)(it / c.nkv), head = (int)(it % c.nkv);
+        const int p = pos[row];
+        const int64_t at = r.cs && (unsigned)p >= (unsigned)r.n_pos ? -1 : page_block(c, seq[row], p, head);
+        if (at < 0) continue;
+        const int t = p & ((1 << c.page_shift) - 1);
+        for (int kv = 0; kv < 2; kv++) {
+            uint8_t* blk = (kv ? c.v : c.k) + at;
+            head_to_lds<XT, A>(kv ? v : k, row * (kv ? ldv : ldk) + (int64_t)head * c.hd, c.hd, kv ? none : r, p, lane, buf);
+            if constexpr (CT == T_MXFP4) {
+                const uint32_t codes = (c.hd / 2) << c.page_shift;
+                if (16 * lane < c.hd) {
+                    float x[2][8];
+#pragma unroll
+                    for (int i = 0; i < 16; i++) x[i / 8][i % 8] = (float)buf[16 * lane + i];
+                    fp4_put(blk, codes, c.hd, t, kv, 16 * lane, 16 * lane + 8, false, x);
+                }
+            } else {
+                typedef typename Elem<CT>::type E;
+                for (int d = lane; d < c.hd; d += 64) ((E*)blk)[t * c.hd + d] = (E)(float)buf[d];
+            }
+            lds_sync_wave();
+        }
+    }
+}
+
+template <int XT, int CT>
+static void launch_append(const KvPages& c, const Rows& k, const Rows& v, const int* seq, const int* pos, int rows,
+                          const RopeArgs& r, hipStream_t s) {
+    const int64_t items = (int64_t)rows * c.nkv;
+    // in the half layout 4-bit blocks of 32 dims have to fall together on either side of rot / 2
+    const bool blocks = CT != T_MXFP4 || !r.cs || r.interleaved || r.rot % 64 == 0;
+    if (units_ok(c.hd, r) && rows16(k) && rows16(v) && blocks)
+        k_kv_append_units<XT, CT><<<unit_grid(items, log2_up(c.hd / 16)), 256, 0, s>>>(c, k.p, v.p, k.ld, v.ld, seq, pos,
+                                                                                       rows, r);
+    else
+        k_kv_append_any<XT, CT><<<(unsigned)std::min<int64_t>(items, 1 << 20), 64, 0, s>>>(c, k.p, v.p, k.ld, v.ld, seq, pos,
+                                                                                         rows, r);
 }
 
 void kv_append(const KvPages& c, const Rows& k, const Rows& v, const int* seq, const int* pos, int rows,
                const RopeArgs& r, hipStream_t s) {
     if (rows <= 0) return;
-    const unsigned grid = (unsigned)rows * c.nkv;
     by_type(k.type, [&](auto xt) {
-        if (c.type == T_MXFP4)
-            k_kv_append<xt(), T_MXFP4><<<grid, 64, 0, s>>>(c, k.p, v.p, k.ld, v.ld, seq, pos, r);
-        else if (c.type == T_F16)
-            k_kv_append<xt(), T_F16><<<grid, 64, 0, s>>>(c, k.p, v.p, k.ld, v.ld, seq, pos, r);
-        else
-            k_kv_append<xt(), T_BF16><<<grid, 64, 0, s>>>(c, k.p, v.p, k.ld, v.ld, seq, pos, r);
+        if (c.type == T_MXFP4) launch_append<xt(), T_MXFP4>(c, k, v, seq, pos, rows, r, s);
+        else if (c.type == T_F16) launch_append<xt(), T_F16>(c, k, v, seq, pos, rows, r, s);
+        else launch_append<xt(), T_BF16>(c, k, v, seq, pos, rows, r, s);
     });
 }
 
-// the value at (token, dim) of a block
+// 8 dims from d on of token t
 template <int CT>
-__device__ __forceinline__ float block_value(const KvPages& c, const uint8_t* blk, bool is_v, int t, int d) {
+__device__ __forceinline__ void block_values(const KvPages& c, const uint8_t* blk, bool is_v, int t, int d, float (&v)[8]) {
     if constexpr (CT == T_MXFP4) {
         const uint32_t codes = (c.hd / 2) << c.page_shift;
-        const uint32_t b = blk[(is_v ? fp4_v_code : fp4_k_code)(c.hd, t, d)];
-        return fp4_value(d & 1 ? b >> 4 : b & 15, blk[codes + (is_v ? fp4_v_scale : fp4_k_scale)(c.hd, t, d)]);
+        uint32_t w;
+        if (is_v && c.hd == 64)
+            w = *(const uint16_t*)(blk + fp4_v_code(c.hd, t, d)) | (uint32_t)*(const uint16_t*)(blk + fp4_v_code(c.hd, t, d + 4)) << 16;
+        else
+            w = *(const uint32_t*)(blk + (is_v ? fp4_v_code : fp4_k_code)(c.hd, t, d));
+        const uint32_t sc = blk[codes + (is_v ? fp4_v_scale : fp4_k_scale)(c.hd, t, d)];
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = fp4_value(w >> (4 * i) & 15, sc);
     } else {
-        return (float)((const typename Elem<CT>::type*)blk)[t * c.hd + d];
+        load8<CT>(blk, (int64_t)t * c.hd + d, v);
+    }
+}
+
+// a thread: 8 dims of K and of V of one KV head
+template <int CT, int YT, bool WIDE>
+__global__ __launch_bounds__(256) void k_kv_gather(KvPages c, const int* __restrict__ seq, const int* __restrict__ pos,
+                                                   int rows, void* k, void* v, int64_t ldk, int64_t ldv) {
+    const int lanes = c.hd / 8, ll = 31 - __builtin_clz(lanes), d = 8 * (threadIdx.x & (lanes - 1));
+    const int64_t items = (int64_t)rows * c.nkv, step = (int64_t)gridDim.x * (256 >> ll);
+    for (int64_t it = (int64_t)blockIdx.x * (256 >> ll) + (threadIdx.x >> ll); it < items; it += step) {
+        const int row = (int)(it / c.nkv), head = (int)(it % c.nkv), p = pos[row];
+        const int64_t at = page_block(c, seq[row], p, head);
+        if (at < 0) continue;
+        const int t = p & ((1 << c.page_shift) - 1);
+#pragma unroll
+        for (int kv = 0; kv < 2; kv++) {
+            void* y = kv ? v : k;
+            if (!y) continue;
+            const int64_t to = row * (kv ? ldv : ldk) + (int64_t)head * c.hd + d;
+            float x[8];
+            block_values<CT>(c, (kv ? c.v : c.k) + at, kv, t, d, x);
+            if constexpr (WIDE) {
+                store8<YT>(y, to, x);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i++) ((typename Elem<YT>::type*)y)[to + i] = (typename Elem<YT>::type)x[i];
+            }
+        }
     }
 }
 
 template <int CT, int YT>
-__global__ __launch_bounds__(64) void k_kv_gather(KvPages c, const int* __restrict__ seq, const int* __restrict__ pos,
-                                                  void* k, void* v, int64_t ldk, int64_t ldv) {
-    const int row = blockIdx.x / c.nkv, head = blockIdx.x % c.nkv;
-    const int p = pos[row];
-    const int64_t at = page_block(c, seq[row], p, head);
-    if (at < 0) return;
-    typedef typename Elem<YT>::type Y;
-    const int t = p & ((1 << c.page_shift) - 1);
-    for (int d = threadIdx.x; d < c.hd; d += 64) {
-        if (k) ((Y*)k)[row * ldk + head * c.hd + d] = (Y)block_value<CT>(c, c.k + at, false, t, d);
-        if (v) ((Y*)v)[row * ldv + head * c.hd + d] = (Y)block_value<CT>(c, c.v + at, true, t, d);
-    }
+static void launch_gather(const KvPages& c, const int* seq, const int* pos, int rows, const Rows& k, const Rows& v,
+                          hipStream_t s) {
+    const unsigned grid = unit_grid((int64_t)rows * c.nkv, log2_up(c.hd / 8));
+    if (rows16(k) && rows16(v))
+        k_kv_gather<CT, YT, true><<<grid, 256, 0, s>>>(c, seq, pos, rows, (void*)k.p, (void*)v.p, k.ld, v.ld);
+    else
+        k_kv_gather<CT, YT, false><<<grid, 256, 0, s>>>(c, seq, pos, rows, (void*)k.p, (void*)v.p, k.ld, v.ld);
 }
 
 void kv_gather(const KvPages& c, const int* seq, const int* pos, int rows, const Rows& k, const Rows& v,
                hipStream_t s) {
     if (rows <= 0) return;
-    const unsigned grid = (unsigned)rows * c.nkv;
     by_type(k.type, [&](auto yt) {
-        if (c.type == T_MXFP4)
-            k_kv_gather<T_MXFP4, yt()><<<grid, 64, 0, s>>>(c, seq, pos, (void*)k.p, (void*)v.p, k.ld, v.ld);
-        else if (c.type == T_F16)
-            k_kv_gather<T_F16, yt()><<<grid, 64, 0, s>>>(c, seq, pos, (void*)k.p, (void*)v.p, k.ld, v.ld);
-        else
-            k_kv_gather<T_BF16, yt()><<<grid, 64, 0, s>>>(c, seq, pos, (void*)k.p, (void*)v.p, k.ld, v.ld);
+        if (c.type == T_MXFP4) launch_gather<T_MXFP4, yt()>(c, seq, pos, rows, k, v, s);
+        else if (c.type == T_F16) launch_gather<T_F16, yt()>(c, seq, pos, rows, k, v, s);
+        else launch_gather<T_BF16, yt()>(c, seq, pos, rows, k, v, s);
     });
 }
 

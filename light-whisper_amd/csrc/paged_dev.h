@@ -45,13 +45,6 @@ __device__ __forceinline__ int fp4_scale(float amax) {
     const int e = (int)(b >> 23) - 127 - ((b & 0x7fffffu) <= 0x400000u ? 2 : 1);
     return min(max(e, -23), 13) + 127;
 }
-// nearest e2m1 code of x · 2^(127 − scale) (the product is exact or far below the first border), ties to even, saturating
-__device__ __forceinline__ uint32_t fp4_code(float x, int scale) {
-    if (scale == 255) return 0;
-    const float a = fabsf(x) * __uint_as_float((uint32_t)(254 - scale) << 23);
-    const uint32_t c = (a > 0.25f) + (a >= 0.75f) + (a > 1.25f) + (a >= 1.75f) + (a > 2.5f) + (a >= 3.5f) + (a > 5.f);
-    return c | (__float_as_uint(x) >> 31) << 3;
-}
 __device__ __forceinline__ float fp4_value(uint32_t code, uint32_t scale) {
     if (scale == 255) return __uint_as_float(0x7fc00000u);
     const uint32_t m = code & 7;
