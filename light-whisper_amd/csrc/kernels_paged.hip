@@ -87,21 +87,36 @@ __device__ void head_to_lds(const void* x, int64_t off, int hd, const RopeArgs& 
 // A thread takes up to four heads of its row with one read of the table.  Bound by memory.
 constexpr int kHeadsPer = 4;
 
+// 8 elements as they were loaded; they are widened only when they are used, so that many loads are in flight
 template <int T>
-__device__ __forceinline__ void load8(const void* p, int64_t at, float (&v)[8]) {
+struct Raw8 {
+    uint4 d[T == T_F32 ? 2 : 1];
+};
+template <int T>
+__device__ __forceinline__ Raw8<T> raw8(const void* p, int64_t at) {
+    Raw8<T> r;
+    const uint4* s = (const uint4*)((const uint8_t*)p + at * (T == T_F32 ? 4 : 2));
+    r.d[0] = s[0];
+    if constexpr (T == T_F32) r.d[1] = s[1];
+    return r;
+}
+template <int T>
+__device__ __forceinline__ void widen8(const Raw8<T>& r, float (&v)[8]) {
     if constexpr (T == T_F32) {
-        const float4 a = *(const float4*)((const float*)p + at), b = *(const float4*)((const float*)p + at + 4);
+        const float4 a = __builtin_bit_cast(float4, r.d[0]), b = __builtin_bit_cast(float4, r.d[1]);
         v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
     } else if constexpr (T == T_F16) {
-        const f16x8 a = *(const f16x8*)((const uint16_t*)p + at);
+        const f16x8 a = __builtin_bit_cast(f16x8, r.d[0]);
 #pragma unroll
         for (int i = 0; i < 8; i++) v[i] = (float)a[i];
     } else {
-        const bf16x8 a = *(const bf16x8*)((const uint16_t*)p + at);
+        const bf16x8 a = __builtin_bit_cast(bf16x8, r.d[0]);
 #pragma unroll
         for (int i = 0; i < 8; i++) v[i] = (float)a[i];
     }
 }
+template <int T>
+__device__ __forceinline__ void load8(const void* p, int64_t at, float (&v)[8]) { widen8<T>(raw8<T>(p, at), v); }
 template <int T>
 __device__ __forceinline__ void store8(void* p, int64_t at, const float (&v)[8]) {
     if constexpr (T == T_F32) {
@@ -201,28 +216,29 @@ __global__ __launch_bounds__(256) void k_rope_units(const void* x, int64_t ldx, 
         const int row = (int)(it / groups), h0 = (int)(it % groups) * HP;
         const int p = r.cs ? pos[row] : 0;
         if (r.cs && (unsigned)p >= (unsigned)r.n_pos) continue;   // the whole group of lanes
-        float cs[16], w[2][8], v[HP][2][8];
+        float cs[16], w[2][8];
+        Raw8<XT> raw[HP][2];
         if (mine) {
-            load_unit_consts(un, r, p, u, cs, w);
 #pragma unroll
-            for (int k = 0; k < HP; k++)
-                if (h0 + k < heads) {
-                    const int64_t at = row * ldx + (int64_t)(h0 + k) * hd;
-                    load8<XT>(x, at + un.a, v[k][0]);
-                    load8<XT>(x, at + un.b, v[k][1]);
-                }
+            for (int k = 0; k < HP; k++) {   // (a head past the last one: the last one again, not stored)
+                const int64_t at = row * ldx + (int64_t)min(h0 + k, heads - 1) * hd;
+                raw[k][0] = raw8<XT>(x, at + un.a);
+                raw[k][1] = raw8<XT>(x, at + un.b);
+            }
+            load_unit_consts(un, r, p, u, cs, w);
         }
 #pragma unroll
         for (int k = 0; k < HP; k++) {
-            if (h0 + k >= heads) break;
-            if (!mine)
-#pragma unroll
-                for (int i = 0; i < 8; i++) v[k][0][i] = v[k][1][i] = 0.f;
-            turn16<float>(v[k], un, r, hd, lanes, cs, w);
+            float v[2][8] = {};
             if (mine) {
+                widen8<XT>(raw[k][0], v[0]);
+                widen8<XT>(raw[k][1], v[1]);
+            }
+            turn16<float>(v, un, r, hd, lanes, cs, w);
+            if (mine && h0 + k < heads) {
                 const int64_t at = row * ldy + (int64_t)(h0 + k) * hd;
-                store8<YT>(y, at + un.a, v[k][0]);
-                store8<YT>(y, at + un.b, v[k][1]);
+                store8<YT>(y, at + un.a, v[0]);
+                store8<YT>(y, at + un.b, v[1]);
             }
         }
     }
