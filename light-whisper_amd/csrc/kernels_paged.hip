@@ -82,9 +82,10 @@ __device__ void head_to_lds(const void* x, int64_t off, int hd, const RopeArgs& 
 }
 
 // ---- the fast form: a thread takes 16 dims of a head, as two runs of 8 with 16-byte accesses: dims 8 u and rot/2 + 8 u in
-// the half layout (each pair in one thread), 16 u and 16 u + 8 in the interleaved one and behind the rotated dims.  The
-// head's hd / 16 threads are neighbours, so a run of lanes reads a run of bytes and the norm's sum is a few xor-shuffles.
-// A thread takes up to four heads of its row with one read of the table.  Bound by memory.
+// the half layout (each pair in one thread), 8 u and hd/2 + 8 u in the interleaved one, and the two halves of the dims that
+// do not rotate likewise.  The head's hd / 16 threads are neighbours, so a run of lanes reads a run of bytes (a lane's 16
+// dims in one piece: a third slower) and the norm's sum is a few xor-shuffles.  A thread takes up to four heads of its row
+// with one read of the table.  Bound by memory.
 constexpr int kHeadsPer = 4;
 
 // 8 elements as they were loaded; they are widened only when they are used, so that many loads are in flight
@@ -137,18 +138,19 @@ __device__ __forceinline__ void store8(void* p, int64_t at, const float (&v)[8])
 // whether rows can be read and written 16 bytes at a time
 static bool rows16(const Rows& r) { return ((uintptr_t)r.p & 15) == 0 && r.ld * elem_bytes(r.type) % 16 == 0; }
 static bool units_ok(int hd, const RopeArgs& r) {
-    return hd % 16 == 0 && (!r.cs || (r.rot % 16 == 0 && ((uintptr_t)r.cs & 15) == 0)) && ((uintptr_t)r.norm_w & 15) == 0;
+    return hd % 16 == 0 && (!r.cs || (r.rot % (r.interleaved ? 8 : 16) == 0 && ((uintptr_t)r.cs & 15) == 0)) && ((uintptr_t)r.norm_w & 15) == 0;
 }
 
 // a thread's place in a head, the same for all rows
 struct Unit {
     int a, b;      // its two runs' first dims
-    bool turn;     // they rotate
+    bool ta, tb;   // which of them rotate
 };
-__device__ __forceinline__ Unit unit_of(int u, const RopeArgs& r) {
+__device__ __forceinline__ Unit unit_of(int u, int hd, const RopeArgs& r) {
     const int n = r.cs ? r.rot / 16 : 0;
-    if (u < n && !r.interleaved) return Unit{8 * u, r.rot / 2 + 8 * u, true};
-    return Unit{16 * u, 16 * u + 8, u < n};
+    if (r.interleaved || n == 0) return Unit{8 * u, hd / 2 + 8 * u, r.cs && 8 * u < r.rot, r.cs && hd / 2 + 8 * u < r.rot};
+    if (u < n) return Unit{8 * u, r.rot / 2 + 8 * u, true, true};
+    return Unit{r.rot + 8 * (u - n), r.rot + (hd - r.rot) / 2 + 8 * (u - n), false, false};
 }
 // norm and rotation of the 16 dims; cs: the row's table entries of the unit (8 of cos, sin), w: its norm weights.
 // `lanes`: threads of a head rounded up to a power of two; those without dims hold zeros
@@ -169,17 +171,17 @@ __device__ __forceinline__ void turn16(A (&x)[2][8], const Unit& un, const RopeA
             x[1][i] = x[1][i] * inv * (A)w[1][i];
         }
     }
-    if (!un.turn) return;
     if (r.interleaved) {
 #pragma unroll
         for (int k = 0; k < 2; k++)
+            if (k ? un.tb : un.ta)
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const A c = cs[8 * k + 2 * i], s = cs[8 * k + 2 * i + 1], u = x[k][2 * i], v = x[k][2 * i + 1];
                 x[k][2 * i] = u * c - v * s;
                 x[k][2 * i + 1] = v * c + u * s;
             }
-    } else {
+    } else if (un.ta) {
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             const A c = cs[2 * i], s = cs[2 * i + 1], u = x[0][i], v = x[1][i];
@@ -188,15 +190,14 @@ __device__ __forceinline__ void turn16(A (&x)[2][8], const Unit& un, const RopeA
         }
     }
 }
-__device__ __forceinline__ void load_unit_consts(const Unit& un, const RopeArgs& r, int p, int u, float (&cs)[16],
+__device__ __forceinline__ void load_unit_consts(const Unit& un, const RopeArgs& r, int p, float (&cs)[16],
                                                  float (&w)[2][8]) {
-    if (un.turn) {
-        const float4* t = (const float4*)(r.cs + ((int64_t)p * (r.rot / 2) + 8 * u) * 2);
+    const float4* row = (const float4*)(r.cs + (int64_t)p * r.rot);   // cos, sin of two pairs each
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const float4 v = t[i];
-            cs[4 * i] = v.x, cs[4 * i + 1] = v.y, cs[4 * i + 2] = v.z, cs[4 * i + 3] = v.w;
-        }
+    for (int i = 0; i < 4; i++) {
+        float4 v = {};
+        if (i < 2 ? un.ta : un.tb) v = row[r.interleaved ? (i < 2 ? un.a : un.b) / 4 + i % 2 : un.a / 2 + i];
+        cs[4 * i] = v.x, cs[4 * i + 1] = v.y, cs[4 * i + 2] = v.z, cs[4 * i + 3] = v.w;
     }
     if (r.norm_w) {
         load8<T_F32>(r.norm_w, un.a, w[0]);
@@ -210,7 +211,7 @@ __global__ __launch_bounds__(256) void k_rope_units(const void* x, int64_t ldx, 
                                                     int heads, int hd, int lanes_log2, RopeArgs r, void* y, int64_t ldy) {
     const int lanes = 1 << lanes_log2, u = threadIdx.x & (lanes - 1), groups = (heads + HP - 1) / HP;
     const bool mine = u < hd / 16;
-    const Unit un = unit_of(u, r);
+    const Unit un = unit_of(u, hd, r);
     const int64_t items = (int64_t)rows * groups, step = (int64_t)gridDim.x * (256 >> lanes_log2);
     for (int64_t it = (int64_t)blockIdx.x * (256 >> lanes_log2) + (threadIdx.x >> lanes_log2); it < items; it += step) {
         const int row = (int)(it / groups), h0 = (int)(it % groups) * HP;
@@ -225,7 +226,7 @@ __global__ __launch_bounds__(256) void k_rope_units(const void* x, int64_t ldx, 
                 raw[k][0] = raw8<XT>(x, at + un.a);
                 raw[k][1] = raw8<XT>(x, at + un.b);
             }
-            load_unit_consts(un, r, p, u, cs, w);
+            load_unit_consts(un, r, p, cs, w);
         }
 #pragma unroll
         for (int k = 0; k < HP; k++) {
@@ -320,20 +321,18 @@ __device__ __forceinline__ uint32_t top8(const float (&v)[8]) {   // the largest
     for (int i = 0; i < 8; i++) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
     return m;
 }
-// two runs of 8 dims (first dims a and b) of token t into an MXFP4 block; `wide`: they lie in blocks of 32 of their own,
-// which 4 neighbouring threads share, else 2 threads' 32 dims are one block
-__device__ __forceinline__ void fp4_put(uint8_t* blk, uint32_t codes, int hd, int t, bool is_v, int a, int b, bool wide,
+// two runs of 8 dims (first dims a and b) of token t into an MXFP4 block; four neighbouring threads' runs are a block of 32
+__device__ __forceinline__ void fp4_put(uint8_t* blk, uint32_t codes, int hd, int t, bool is_v, int a, int b,
                                         const float (&x)[2][8]) {
-    uint32_t m0 = top8(x[0]), m1 = top8(x[1]);
-    const uint32_t both = max(m0, m1);
-    if (!wide) m0 = m1 = both;
-    m0 = max(m0, (uint32_t)__shfl_xor((int)m0, 1));
-    m1 = max(m1, (uint32_t)__shfl_xor((int)m1, 1));
-    const uint32_t n0 = max(m0, (uint32_t)__shfl_xor((int)m0, 2)), n1 = max(m1, (uint32_t)__shfl_xor((int)m1, 2));
-    if (wide) m0 = n0, m1 = n1;
+    uint32_t m[2] = {top8(x[0]), top8(x[1])};
 #pragma unroll
     for (int k = 0; k < 2; k++) {
-        const int d = k ? b : a, sc = fp4_scale(__uint_as_float(k ? m1 : m0));
+        m[k] = max(m[k], (uint32_t)__shfl_xor((int)m[k], 1));
+        m[k] = max(m[k], (uint32_t)__shfl_xor((int)m[k], 2));
+    }
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const int d = k ? b : a, sc = fp4_scale(__uint_as_float(m[k]));
         const uint32_t w = fp4_codes8(x[k], sc);
         if (is_v && hd == 64) {   // 4 dims lie together
             *(uint16_t*)(blk + fp4_v_code(hd, t, d)) = (uint16_t)w;
@@ -353,7 +352,8 @@ __global__ __launch_bounds__(256) void k_kv_append_units(KvPages c, const void* 
     // 4-bit pages: K in 64 bits up to the rounding to f32, so that a value next to a border between two codes gets its own
     typedef typename std::conditional<CT == T_MXFP4, double, float>::type A;
     const int lanes = c.hd / 16, ll = 31 - __builtin_clz(lanes), u = threadIdx.x & (lanes - 1);
-    const Unit un = unit_of(u, r);
+    const Unit un = unit_of(u, c.hd, r);
+    const int va0 = 8 * u, vb0 = c.hd / 2 + 8 * u;   // V's runs
     const int64_t items = (int64_t)rows * c.nkv, step = (int64_t)gridDim.x * (256 >> ll);
     const uint32_t codes = (c.hd / 2) << c.page_shift;
     for (int64_t it = (int64_t)blockIdx.x * (256 >> ll) + (threadIdx.x >> ll); it < items; it += step) {
@@ -365,9 +365,9 @@ __global__ __launch_bounds__(256) void k_kv_append_units(KvPages c, const void* 
         const int64_t ka = row * ldk + (int64_t)head * c.hd, va = row * ldv + (int64_t)head * c.hd;
         load8<XT>(k, ka + un.a, kx[0]);
         load8<XT>(k, ka + un.b, kx[1]);
-        load8<XT>(v, va + 16 * u, vx[0]);
-        load8<XT>(v, va + 16 * u + 8, vx[1]);
-        load_unit_consts(un, r, p, u, cs, w);
+        load8<XT>(v, va + va0, vx[0]);
+        load8<XT>(v, va + vb0, vx[1]);
+        load_unit_consts(un, r, p, cs, w);
         A x[2][8];
 #pragma unroll
         for (int i = 0; i < 8; i++) x[0][i] = kx[0][i], x[1][i] = kx[1][i];
@@ -376,13 +376,13 @@ __global__ __launch_bounds__(256) void k_kv_append_units(KvPages c, const void* 
         for (int i = 0; i < 8; i++) kx[0][i] = (float)x[0][i], kx[1][i] = (float)x[1][i];
         const int t = p & ((1 << c.page_shift) - 1);
         if constexpr (CT == T_MXFP4) {
-            fp4_put(c.k + at, codes, c.hd, t, false, un.a, un.b, un.turn && !r.interleaved, kx);
-            fp4_put(c.v + at, codes, c.hd, t, true, 16 * u, 16 * u + 8, false, vx);
+            fp4_put(c.k + at, codes, c.hd, t, false, un.a, un.b, kx);
+            fp4_put(c.v + at, codes, c.hd, t, true, va0, vb0, vx);
         } else {
             store8<CT>(c.k + at, (int64_t)t * c.hd + un.a, kx[0]);
             store8<CT>(c.k + at, (int64_t)t * c.hd + un.b, kx[1]);
-            store8<CT>(c.v + at, (int64_t)t * c.hd + 16 * u, vx[0]);
-            store8<CT>(c.v + at, (int64_t)t * c.hd + 16 * u + 8, vx[1]);
+            store8<CT>(c.v + at, (int64_t)t * c.hd + va0, vx[0]);
+            store8<CT>(c.v + at, (int64_t)t * c.hd + vb0, vx[1]);
         }
     }
 }
@@ -410,8 +410,8 @@ __global__ __launch_bounds__(64) void k_kv_append_any(KvPages c, const void* k, 
                 if (16 * lane < c.hd) {
                     float x[2][8];
 #pragma unroll
-                    for (int i = 0; i < 16; i++) x[i / 8][i % 8] = (float)buf[16 * lane + i];
-                    fp4_put(blk, codes, c.hd, t, kv, 16 * lane, 16 * lane + 8, false, x);
+                    for (int i = 0; i < 16; i++) x[i / 8][i % 8] = (float)buf[i / 8 * (c.hd / 2) + 8 * lane + i % 8];
+                    fp4_put(blk, codes, c.hd, t, kv, 8 * lane, c.hd / 2 + 8 * lane, x);
                 }
             } else {
                 typedef typename Elem<CT>::type E;
