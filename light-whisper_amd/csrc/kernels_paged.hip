@@ -46,6 +46,12 @@ __device__ __forceinline__ float shfl_xor_t<float>(float v, int o) { return __sh
 template <>
 __device__ __forceinline__ double shfl_xor_t<double>(double v, int o) { return __shfl_xor(v, o); }
 
+template <typename A>
+__device__ __forceinline__ A fma_t(A a, A b, A c) {
+    if constexpr (sizeof(A) == 8) return fma(a, b, c);
+    else return fmaf(a, b, c);
+}
+
 __device__ __forceinline__ void lds_sync_wave() {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -160,7 +166,7 @@ __device__ __forceinline__ void turn16(A (&x)[2][8], const Unit& un, const RopeA
     if (r.norm_w) {
         A ss = 0;
 #pragma unroll
-        for (int i = 0; i < 8; i++) ss += x[0][i] * x[0][i] + x[1][i] * x[1][i];
+        for (int i = 0; i < 8; i++) ss = fma_t<A>(x[0][i], x[0][i], fma_t<A>(x[1][i], x[1][i], ss));
         for (int o = lanes >> 1; o > 0; o >>= 1) ss += shfl_xor_t<A>(ss, o);
         A inv;
         if constexpr (sizeof(A) == 8) inv = 1.0 / sqrt(ss / (double)hd + (double)r.eps);
@@ -178,15 +184,15 @@ __device__ __forceinline__ void turn16(A (&x)[2][8], const Unit& un, const RopeA
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const A c = cs[8 * k + 2 * i], s = cs[8 * k + 2 * i + 1], u = x[k][2 * i], v = x[k][2 * i + 1];
-                x[k][2 * i] = u * c - v * s;
-                x[k][2 * i + 1] = v * c + u * s;
+                x[k][2 * i] = fma_t<A>(u, c, -(v * s));
+                x[k][2 * i + 1] = fma_t<A>(v, c, u * s);
             }
     } else if (un.ta) {
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             const A c = cs[2 * i], s = cs[2 * i + 1], u = x[0][i], v = x[1][i];
-            x[0][i] = u * c - v * s;
-            x[1][i] = v * c + u * s;
+            x[0][i] = fma_t<A>(u, c, -(v * s));
+            x[1][i] = fma_t<A>(v, c, u * s);
         }
     }
 }
@@ -338,13 +344,14 @@ __device__ __forceinline__ void fp4_put(uint8_t* blk, uint32_t codes, int hd, in
             *(uint16_t*)(blk + fp4_v_code(hd, t, d)) = (uint16_t)w;
             *(uint16_t*)(blk + fp4_v_code(hd, t, d + 4)) = (uint16_t)(w >> 16);
         } else {
-            *(uint32_t*)(blk + (is_v ? fp4_v_code : fp4_k_code)(hd, t, d)) = w;
+            *(uint32_t*)(blk + (is_v ? fp4_v_code(hd, t, d) : fp4_k_code(hd, t, d))) = w;
         }
-        if (d % 32 == 0) blk[codes + (is_v ? fp4_v_scale : fp4_k_scale)(hd, t, d)] = (uint8_t)sc;
+        if (d % 32 == 0) blk[codes + (is_v ? fp4_v_scale(hd, t, d) : fp4_k_scale(hd, t, d))] = (uint8_t)sc;
     }
 }
 
-// a thread: 16 dims of K and of V of one KV head (as k_rope_units; hd is a power of two, so every thread has dims)
+// a thread: 16 dims of K (even waves) or V (odd ones) of one KV head, as k_rope_units; hd is a power of two, so every thread
+// has dims.  (K and V in one thread: with K in 64 bits, 154 registers, a third of the waves and a third more time)
 template <int XT, int CT>
 __global__ __launch_bounds__(256) void k_kv_append_units(KvPages c, const void* k, const void* v, int64_t ldk, int64_t ldv,
                                                          const int* __restrict__ seq, const int* __restrict__ pos, int rows,
@@ -352,37 +359,42 @@ __global__ __launch_bounds__(256) void k_kv_append_units(KvPages c, const void* 
     // 4-bit pages: K in 64 bits up to the rounding to f32, so that a value next to a border between two codes gets its own
     typedef typename std::conditional<CT == T_MXFP4, double, float>::type A;
     const int lanes = c.hd / 16, ll = 31 - __builtin_clz(lanes), u = threadIdx.x & (lanes - 1);
-    const Unit un = unit_of(u, c.hd, r);
-    const int va0 = 8 * u, vb0 = c.hd / 2 + 8 * u;   // V's runs
-    const int64_t items = (int64_t)rows * c.nkv, step = (int64_t)gridDim.x * (256 >> ll);
+    const bool is_v = threadIdx.x >> 6 & 1;
+    const int64_t items = (int64_t)rows * c.nkv, step = (int64_t)gridDim.x * (128 >> ll);
     const uint32_t codes = (c.hd / 2) << c.page_shift;
-    for (int64_t it = (int64_t)blockIdx.x * (256 >> ll) + (threadIdx.x >> ll); it < items; it += step) {
+    const int mine = (threadIdx.x >> 7) * (64 >> ll) + ((threadIdx.x & 63) >> ll);
+    for (int64_t it = (int64_t)blockIdx.x * (128 >> ll) + mine; it < items; it += step) {
         const int row = (int)(it / c.nkv), head = (int)(it % c.nkv);
         const int p = pos[row];
         const int64_t at = r.cs && (unsigned)p >= (unsigned)r.n_pos ? -1 : page_block(c, seq[row], p, head);
         if (at < 0) continue;   // the whole group of lanes
-        float cs[16], w[2][8], kx[2][8], vx[2][8];
-        const int64_t ka = row * ldk + (int64_t)head * c.hd, va = row * ldv + (int64_t)head * c.hd;
-        load8<XT>(k, ka + un.a, kx[0]);
-        load8<XT>(k, ka + un.b, kx[1]);
-        load8<XT>(v, va + va0, vx[0]);
-        load8<XT>(v, va + vb0, vx[1]);
-        load_unit_consts(un, r, p, cs, w);
-        A x[2][8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) x[0][i] = kx[0][i], x[1][i] = kx[1][i];
-        turn16<A>(x, un, r, c.hd, lanes, cs, w);
-#pragma unroll
-        for (int i = 0; i < 8; i++) kx[0][i] = (float)x[0][i], kx[1][i] = (float)x[1][i];
         const int t = p & ((1 << c.page_shift) - 1);
-        if constexpr (CT == T_MXFP4) {
-            fp4_put(c.k + at, codes, c.hd, t, false, un.a, un.b, kx);
-            fp4_put(c.v + at, codes, c.hd, t, true, va0, vb0, vx);
+        const Unit un = is_v ? Unit{8 * u, c.hd / 2 + 8 * u, false, false} : unit_of(u, c.hd, r);
+        const void* src = is_v ? v : k;
+        const int64_t from = row * (is_v ? ldv : ldk) + (int64_t)head * c.hd;
+        const Raw8<XT> raw[2] = {raw8<XT>(src, from + un.a), raw8<XT>(src, from + un.b)};
+        float y[2][8];
+        if (is_v) {
+            widen8<XT>(raw[0], y[0]);
+            widen8<XT>(raw[1], y[1]);
         } else {
-            store8<CT>(c.k + at, (int64_t)t * c.hd + un.a, kx[0]);
-            store8<CT>(c.k + at, (int64_t)t * c.hd + un.b, kx[1]);
-            store8<CT>(c.v + at, (int64_t)t * c.hd + va0, vx[0]);
-            store8<CT>(c.v + at, (int64_t)t * c.hd + vb0, vx[1]);
+            float cs[16], w[2][8];
+            load_unit_consts(un, r, p, cs, w);
+            widen8<XT>(raw[0], y[0]);
+            widen8<XT>(raw[1], y[1]);
+            A x[2][8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[0][i] = y[0][i], x[1][i] = y[1][i];
+            turn16<A>(x, un, r, c.hd, lanes, cs, w);
+#pragma unroll
+            for (int i = 0; i < 8; i++) y[0][i] = (float)x[0][i], y[1][i] = (float)x[1][i];
+        }
+        uint8_t* blk = (is_v ? c.v : c.k) + at;
+        if constexpr (CT == T_MXFP4) {
+            fp4_put(blk, codes, c.hd, t, is_v, un.a, un.b, y);
+        } else {
+            store8<CT>(blk, (int64_t)t * c.hd + un.a, y[0]);
+            store8<CT>(blk, (int64_t)t * c.hd + un.b, y[1]);
         }
     }
 }
@@ -429,7 +441,7 @@ static void launch_append(const KvPages& c, const Rows& k, const Rows& v, const 
     // in the half layout 4-bit blocks of 32 dims have to fall together on either side of rot / 2
     const bool blocks = CT != T_MXFP4 || !r.cs || r.interleaved || r.rot % 64 == 0;
     if (units_ok(c.hd, r) && rows16(k) && rows16(v) && blocks)
-        k_kv_append_units<XT, CT><<<unit_grid(items, log2_up(c.hd / 16)), 256, 0, s>>>(c, k.p, v.p, k.ld, v.ld, seq, pos,
+        k_kv_append_units<XT, CT><<<unit_grid(2 * items, log2_up(c.hd / 16)), 256, 0, s>>>(c, k.p, v.p, k.ld, v.ld, seq, pos,
                                                                                        rows, r);
     else
         k_kv_append_any<XT, CT><<<(unsigned)std::min<int64_t>(items, 1 << 20), 64, 0, s>>>(c, k.p, v.p, k.ld, v.ld, seq, pos,
@@ -455,8 +467,8 @@ __device__ __forceinline__ void block_values(const KvPages& c, const uint8_t* bl
         if (is_v && c.hd == 64)
             w = *(const uint16_t*)(blk + fp4_v_code(c.hd, t, d)) | (uint32_t)*(const uint16_t*)(blk + fp4_v_code(c.hd, t, d + 4)) << 16;
         else
-            w = *(const uint32_t*)(blk + (is_v ? fp4_v_code : fp4_k_code)(c.hd, t, d));
-        const uint32_t sc = blk[codes + (is_v ? fp4_v_scale : fp4_k_scale)(c.hd, t, d)];
+            w = *(const uint32_t*)(blk + (is_v ? fp4_v_code(c.hd, t, d) : fp4_k_code(c.hd, t, d)));
+        const uint32_t sc = blk[codes + (is_v ? fp4_v_scale(c.hd, t, d) : fp4_k_scale(c.hd, t, d))];
 #pragma unroll
         for (int i = 0; i < 8; i++) v[i] = fp4_value(w >> (4 * i) & 15, sc);
     } else {
