@@ -543,7 +543,7 @@ def test_steps_of_a_session_batch(torch_dev, kv):
     slots = int((lens + steps).sum())
     flat = [torch.zeros((slots, nkv * hd), dtype=torch.float16, device="cuda:0") for _ in range(2)]
     base = np.array([0, lens[0] + steps])
-    ws = torch.zeros(1 << 26, dtype=torch.uint8, device="cuda:0")
+    ws = torch.zeros(1 << 27, dtype=torch.uint8, device="cuda:0")
     for step in range(steps + 1):
         new = lens if step == 0 else np.ones(2, np.int64)
         rows = int(new.sum())
