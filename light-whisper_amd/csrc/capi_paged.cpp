@@ -219,7 +219,7 @@ QASR_API int qasr_op_paged_attention(const qasr_kv_cache* c, const qasr_paged_at
         QASR_CHECK(q && o && q_start && kv_len && aligned(q_start, 4) && aligned(kv_len, 4), QASR_E_INVALID,
                    "paged_attention: NULL argument");
         const size_t need = paged_attention_ws(p, at);
-        QASR_CHECK(need == 0 || (ws && aligned(ws, 16) && ws_bytes >= need), QASR_E_CAPACITY,
+        QASR_CHECK(need == 0 || (ws && aligned(ws, 128) && ws_bytes >= need), QASR_E_CAPACITY,
                    "paged_attention: the workspace is smaller than qasr_paged_attention_workspace says, or misaligned");
         paged_attention(p, at, q, ldq, q_start, kv_len, rows, o, ldo, ws, stream_of(stream));
         QASR_HIP(hipGetLastError());

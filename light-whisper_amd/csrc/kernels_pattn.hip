@@ -693,6 +693,9 @@ __global__ __launch_bounds__(256, wgs_per_cu(HD, CT)) void k_paged_attn(KvPages 
 // different XCDs: with 8 heads an XCD's L2 serves one).  Where the items are too few for the chip, `splits` workgroups
 // share one item's keys and the last to arrive joins their parts.
 constexpr int kRowBlock = 128, kPromptKeys = 64;
+constexpr int kPromptSlots = 1024;   // parts of all items together where items are split
+// parts of one item at most, and tiles of a part at least: the last to arrive reads the others' 64 KB each, about 1 us
+constexpr int kPromptParts = 32, kPartTiles = 8;
 
 template <int HD>
 __device__ __forceinline__ int k_swz(int row) { return row & (HD / 8 - 1); }
@@ -750,7 +753,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_paged_prompt(
     const int blk_hi = a.causal ? max(0, min(x.len, p0 + row_base / G + 1)) : x.len;
     const int blk_lo = a.window > 0 ? max(0, p0 + (row_base + nrow - 1) / G - a.window + 1) : 0;
     const int tile0 = b_lo / kPromptKeys, tiles = max(0, (b_hi + kPromptKeys - 1) / kPromptKeys - tile0);
-    const int parts = max(1, min(splits, tiles));   // with at least one tile each
+    const int parts = max(1, min(splits, tiles / kPartTiles));
     if (split >= parts) return;
     const int t_begin = tile0 + (int)((int64_t)tiles * split / parts), t_end = tile0 + (int)((int64_t)tiles * (split + 1) / parts);
 
@@ -1060,15 +1063,17 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_paged_prompt(
         const int item_slot = item * splits;
         float* mine = part + (int64_t)(item_slot + split) * kSlot;
         const uint32_t off = ((w * DT * 4) * 64 + lane) * 16;
+        if (wrows > 0) {
 #pragma unroll
-        for (int dt = 0; dt < DT; dt++)
+            for (int dt = 0; dt < DT; dt++)
 #pragma unroll
-            for (int g = 0; g < 4; g++)
-                wt_st128(mine, off + (dt * 4 + g) * 1024,
-                         __builtin_bit_cast(wt_v4i, f32x4{acc[dt][4 * g], acc[dt][4 * g + 1], acc[dt][4 * g + 2], acc[dt][4 * g + 3]}));
-        if (h == 0) {
-            wt_stf(mine, (kRowBlock * HD + 32 * w + n) * 4, m);
-            wt_stf(mine, (kRowBlock * (HD + 1) + 32 * w + n) * 4, l);
+                for (int g = 0; g < 4; g++)
+                    wt_st128(mine, off + (dt * 4 + g) * 1024,
+                             __builtin_bit_cast(wt_v4i, f32x4{acc[dt][4 * g], acc[dt][4 * g + 1], acc[dt][4 * g + 2], acc[dt][4 * g + 3]}));
+            if (h == 0) {
+                wt_stf(mine, (kRowBlock * HD + 32 * w + n) * 4, m);
+                wt_stf(mine, (kRowBlock * (HD + 1) + 32 * w + n) * 4, l);
+            }
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // written through before the arrival is counted
         __syncthreads();
@@ -1086,7 +1091,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_paged_prompt(
             for (int i = 0; i < DT; i++)
 #pragma unroll
                 for (int j = 0; j < 16; j++) acc[i][j] = 0.f;
-            for (int pc = 0; pc < parts; pc++) {
+            for (int pc = 0; pc < (wrows > 0 ? parts : 0); pc++) {
                 const float* src = part + (int64_t)(item_slot + pc) * kSlot;
                 const float f = __builtin_amdgcn_exp2f(wt_ldf(src, (kRowBlock * HD + 32 * w + n) * 4) - M);
                 l = fmaf(wt_ldf(src, (kRowBlock * (HD + 1) + 32 * w + n) * 4), f, l);
@@ -1119,9 +1124,14 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_paged_prompt(
 
 }  // namespace
 
-// which kernel: prompts fill 32-row matrix tiles, single tokens and short verify passes do not
-static bool is_prompt(const KvPages& c, const AttnArgs& a) { return (int64_t)a.max_q * (a.nh / c.nkv) > 32; }
-constexpr int kPromptSlots = 1024;   // parts at most where items are split
+// Which kernel, by the rows (tokens · heads of a KV head) of a sequence.  The few-row one reads the keys anew for every 16
+// rows, which L2 bears for a while; the prompt one has whole blocks of 128 rows to fill and more to start.  Measured (f16,
+// one sequence of 32,768 keys, 16 / 8 heads): 64 rows 58 against 64 us, 128 rows 90 against 66; over 4-bit pages, a quarter of
+// the bytes, 256 rows 105 against 89 us (32 x 4,096 keys: 93 against 100); 2,000 keys: 256 rows 20 against 36 us
+static bool is_prompt(const KvPages& c, const AttnArgs& a) {
+    const int64_t few = c.type == T_MXFP4 || a.max_kv <= 2048 ? 256 : 64;
+    return (int64_t)a.max_q * (a.nh / c.nkv) > few;
+}
 
 size_t paged_attention_ws(const KvPages& c, const AttnArgs& a) {
     const size_t few = (size_t)kSplitWgs * 4 + (size_t)kSplitWgs * 2 * (16 * c.hd + 32) * 4;
@@ -1140,15 +1150,10 @@ static void launch(const KvPages& c, const AttnArgs& a, const void* q, int64_t l
     if (is_prompt(c, a)) {
         const int64_t items = ((int64_t)rows * G / kRowBlock + c.n_seq) * c.nkv;   // at most
         QASR_CHECK(items < 1 << 23, QASR_E_CAPACITY, "paged_attention: too many rows for one call");
-        const int splits = (int)std::max<int64_t>(1, kPromptSlots / items);
+        const int splits = (int)std::min<int64_t>(kPromptParts, std::max<int64_t>(1, kPromptSlots / items));
         const size_t lds = 4 * kPromptKeys * HD * 2;
-        if (lds > 65536) {
-            static const bool set = [&] {
-                QASR_HIP(hipFuncSetAttribute((const void*)k_paged_prompt<HD, CT, QT>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-                return true;
-            }();
-            (void)set;
-        }
+        if constexpr (HD == 256)   // (for the current device; past 64 KB)
+            QASR_HIP(hipFuncSetAttribute((const void*)k_paged_prompt<HD, CT, QT>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
         k_paged_prompt<HD, CT, QT><<<(unsigned)(items * splits), 256, lds, s>>>(c, a, q, ldq, q_start, kv_len, rows, o, ldo,
                                                                                part, cnt, splits, q_vec, o_vec);
         return;

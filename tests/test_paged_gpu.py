@@ -364,8 +364,9 @@ def test_attention_prompts(torch_dev, kv, qt, causal, window, nkv, g, hd, page):
     rng = np.random.default_rng(nkv * hd + g)
     for lens, nq in (([5], [5]), ([40, 200, 3, 70], [40, 33, 3, 9]), ([10, 0, 90], [17, 4, 90]), ([300], [131])):
         c, q, qs, kl = make(rng, kv, page, nkv, g, hd, lens, nq, qt)
-        o = attend(c, q, qs, kl, nkv * g, causal, window, hd ** -0.5)
-        check_attend(c, q, o, qs, kl, nkv * g, causal, window, hd ** -0.5, qt, qt)
+        for hints in ((None, None), (1000, 1 << 20)):     # either way of splitting the work
+            o = attend(c, q, qs, kl, nkv * g, causal, window, hd ** -0.5, max_q=hints[0], max_kv=hints[1])
+            check_attend(c, q, o, qs, kl, nkv * g, causal, window, hd ** -0.5, qt, qt)
 
 
 @pytest.mark.parametrize("kv,qt", LAYOUTS)
@@ -374,10 +375,11 @@ def test_attention_long(torch_dev, kv, qt):
     rng = np.random.default_rng(8)
     for lens, nq in (([9001], [1]), ([5000, 3, 40, 1], [1, 1, 1, 1]), ([4097, 700], [6, 5]), ([6000] + [30] * 40, [1] * 41)):
         c, q, qs, kl = make(rng, kv, 64, 2, 2, 128, lens, nq, qt)
-        o = attend(c, q, qs, kl, 4, True, 0, 0.09)
-        check_attend(c, q, o, qs, kl, 4, True, 0, 0.09, qt, qt)
-        again = attend(c, q, qs, kl, 4, True, 0, 0.09)
-        assert c.torch.equal(o, again)
+        for max_q in (None, 1000):     # either way of splitting the work
+            o = attend(c, q, qs, kl, 4, True, 0, 0.09, max_q=max_q)
+            check_attend(c, q, o, qs, kl, 4, True, 0, 0.09, qt, qt)
+            again = attend(c, q, qs, kl, 4, True, 0, 0.09, max_q=max_q)
+            assert c.torch.equal(o, again)
 
 
 @pytest.mark.parametrize("kv,qt", LAYOUTS)
@@ -388,9 +390,9 @@ def test_attention_f32_output_and_strides(torch_dev, kv, qt):
     c, _, qs, kl = make(rng, kv, 32, 2, 2, 128, [100, 7], [40, 1], qt)
     for ldq, ldo in ((4 * 128 + 8, 4 * 128 + 4), (4 * 128 + 1, 4 * 128 + 3)):
         q = dev(rng.standard_normal((41, ldq)).astype(np.float32), qt)
-        for ot in ("f32", qt):
+        for ot, max_q in (("f32", 1), (qt, 1), ("f32", 1000), (qt, 1000)):
             o = torch.full((41, ldo), 9.0, device="cuda:0", dtype=T(ot))
-            attend(c, q, qs, kl, 4, True, 0, 0.1, ot=ot, o=o)
+            attend(c, q, qs, kl, 4, True, 0, 0.1, ot=ot, o=o, max_q=max_q)
             check_attend(c, q, o, qs, kl, 4, True, 0, 0.1, qt, ot)
             assert (num(o)[:, 512:] == 9).all()
 
@@ -424,12 +426,12 @@ def test_attention_nothing_outside_the_keys(torch_dev, kv, qt, nq):
             p.copy_(torch.from_numpy(raw))
         else:
             p[~keep.to("cuda:0")[:, None].expand(-1, 2, -1)] = float("nan")
-    for hints in ((None, None), (0, 0), (1 << 20, 1 << 30)):
+    for hints in ((None, None), (0, 0), (1 << 20, 1 << 30), (1000, 10 ** 4)):
         o = attend(c, q, qs, kl, 4, True, 0, 0.09, max_q=hints[0], max_kv=hints[1])
         check_attend(c, q, o, qs, kl, 4, True, 0, 0.09, qt, qt, values=clean)
         assert (num(o)[rows:] == 9).all()
     # NaN in the last key: only the rows that see it take it (in either way of splitting the work)
-    before = [num(attend(c, q, qs, kl, 4, True, 0, 0.09, max_q=m)) for m in (1, 1000)]
+    before = [num(attend(c, q, qs, kl, 4, True, 0, 0.09, max_q=m)) for m in (1, 1000)]     # 1,000: as prompts
     ids, t = c.table_h[2, 199 // 16], 199 % 16
     for j, p in enumerate(c.pools):
         if kv == "mxfp4":
@@ -463,8 +465,8 @@ def test_attention_extreme_scores(torch_dev, kv, qt):
     """one key far above the others, scores of the same size, a zero scale, large values"""
     rng = np.random.default_rng(12)
     c, q, qs, kl = make(rng, kv, 32, 2, 2, 128, [400, 90], [1, 50], qt)
-    for scale in (0.0, 30.0, -2.0):
-        o = attend(c, q, qs, kl, 4, True, 0, scale)
+    for scale, max_q in ((0.0, 1), (30.0, 1), (-2.0, 1), (0.0, 1000), (30.0, 1000), (-2.0, 1000)):
+        o = attend(c, q, qs, kl, 4, True, 0, scale, max_q=max_q)
         check_attend(c, q, o, qs, kl, 4, True, 0, scale, qt, qt)
     if kv == "mxfp4":
         hd, page = 128, 32
@@ -472,9 +474,26 @@ def test_attention_extreme_scores(torch_dev, kv, qt):
     else:
         c.pools[1].mul_(20000.0 if kv == "f16" else 1e30)
         c.pools[1].clamp_(-60000 if kv == "f16" else -1e38, 60000 if kv == "f16" else 1e38)
-    for scale in (0.01, 0.3):
-        o = attend(c, q, qs, kl, 4, True, 0, scale, ot="f32")
+    for scale, max_q in ((0.01, 1), (0.3, 1), (0.01, 1000), (0.3, 1000)):
+        o = attend(c, q, qs, kl, 4, True, 0, scale, ot="f32", max_q=max_q)
         check_attend(c, q, o, qs, kl, 4, True, 0, scale, qt, "f32")
+
+
+@pytest.mark.parametrize("kv,qt", LAYOUTS)
+def test_attention_small_values(torch_dev, kv, qt):
+    """K and V in the range where f16 has no leading one left (and the smallest scales of 4-bit pages): nothing is flushed"""
+    rng = np.random.default_rng(17)
+    c, q, qs, kl = make(rng, kv, 32, 2, 2, 128, [300, 45], [1, 45], qt)
+    if kv == "mxfp4":
+        for p in c.pools:
+            p[:, :, 32 * 64:] = dev(rng.integers(104, 108, (c.n_pages, 2, 32 * 4)).astype(np.uint8))
+    else:
+        for p in c.pools:
+            p.mul_(2.0 ** -16)
+    for max_q in (1, 1000):
+        o = attend(c, q, qs, kl, 4, True, 0, 3e4, ot="f32", max_q=max_q)
+        check_attend(c, q, o, qs, kl, 4, True, 0, 3e4, qt, "f32")
+        assert (o[kl.argmax()] != 0).any()
 
 
 @pytest.mark.parametrize("kv,qt", LAYOUTS)
@@ -483,8 +502,9 @@ def test_attention_many_sequences(torch_dev, kv, qt):
     lens = rng.integers(0, 90, 300)
     nq = rng.integers(0, 4, 300)
     c, q, qs, kl = make(rng, kv, 16, 1, 2, 64, lens, nq, qt)
-    o = attend(c, q, qs, kl, 2, True, 0, 0.12)
-    check_attend(c, q, o, qs, kl, 2, True, 0, 0.12, qt, qt)
+    for max_q in (None, 1000):
+        o = attend(c, q, qs, kl, 2, True, 0, 0.12, max_q=max_q)
+        check_attend(c, q, o, qs, kl, 2, True, 0, 0.12, qt, qt)
 
 
 @pytest.mark.parametrize("kv", ["f16", "mxfp4"])
@@ -514,7 +534,7 @@ def test_offsets_past_32_bits(torch_dev, kv):
     else:
         ks, vs = (x.astype(np.float16).astype(np.float64) for x in (ks, vs))
     assert np.array_equal(num(out[0]), ks) and np.array_equal(num(out[1]), vs)
-    for nq in (1, 40):
+    for nq in (1, 200):
         q = dev(rng.standard_normal((nq, 16 * hd)).astype(np.float32), "f16")
         o = attend(c, q, [0, nq], [n], 16, True, 0, 0.09)
         c2 = Cache(rng, "f16", page, nkv, hd, [1])      # the same values in three pages near the start, for the oracle
