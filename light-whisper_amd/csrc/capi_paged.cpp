@@ -211,7 +211,8 @@ QASR_API int qasr_op_paged_attention(const qasr_kv_cache* c, const qasr_paged_at
     return guard([&] {
         const KvPages p = pages_of(c, true);
         const AttnArgs at = attn_of(p, a);
-        QASR_CHECK(rows >= 0 && (int64_t)rows * at.nh <= INT_MAX, QASR_E_INVALID, "paged_attention: bad row count");
+        QASR_CHECK(rows >= 0 && (int64_t)rows * at.nh <= 1 << 30, QASR_E_INVALID,
+                   "paged_attention: rows * n_heads must be at most 2^30");
         const int64_t w = (int64_t)at.nh * p.hd;
         rows_of(q, at.q_type, ldq, w, rows, "paged_attention: q");
         rows_of(o, at.o_type, ldo, w, rows, "paged_attention: o");

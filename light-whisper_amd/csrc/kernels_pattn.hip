@@ -1,12 +1,18 @@
 // Attention over a paged K/V cache (include/qasr.h, qasr_op_paged_attention), gfx950.
 //
 // Query rows of one sequence and KV head are numbered r = token · G + g (G query heads share a KV head), so that every K/V
-// byte that is loaded serves all G heads, and taken 16 at a time as the columns of v_mfma_f32_16x16x32:
-//   Sᵀ = K·Qᵀ   (16 keys × 16 rows; a lane holds 4 keys of ONE row, so the softmax needs no cross-lane work but a vote)
-//   Oᵀ = Vᵀ·Pᵀ  (16 dims × 16 rows; the lane's 8 weights of 32 keys are the B operand as they stand: contraction slot
-//                (lane >> 4, j) stands for key 16 (j >> 2) + 4 (lane >> 4) + (j & 3), and V is loaded to match)
-// No K/V byte passes LDS: K rows are loaded in the A operand's layout; a lane loads hd/16 dims of its 8 keys of V and
-// pairs them key by key in registers (v_perm), which makes MFMA row m of tile t dim (hd/16) m + t.
+// byte that is loaded serves all G heads, and are the columns of the matrix instructions:
+//   Sᵀ = K·Qᵀ   (keys × rows; a lane holds scores of ONE row, so the softmax needs no cross-lane work but a vote)
+//   Oᵀ = Vᵀ·Pᵀ  (dims × rows; a lane's weights are the second operand as they stand, V is brought to match)
+// One pass over the keys with a running maximum that moves only where some row's rises by more than 2^kSlack: weights are
+// exp2(s − m + kUp), sums and Oᵀ in f32.  Roundings: the weights to q's type for the product with V (half a step each; f16
+// reaches 2^-26 of the largest before its steps stop shrinking), the output to its type.  e2m1 · 2^E is exact in either type.
+//
+// Few rows (k_paged_attn): bound by memory.  16 / 8 heads of 128, f16: one sequence of 32,768 keys 32 us (134 MB, 4.1 TB/s),
+// 64 of 17 .. 8,200 92 us (396 MB, 4.3 TB/s); over 4-bit pages 32 of 501 .. 32,768 76 us (322 MB, 4.2 TB/s; a copy of
+// 2 GiB runs at 4.8).  A token of one sequence of 403 keys: 9 us, all of it round trips.
+// Many rows (k_paged_prompt): bound by the matrix unit and the softmax in turn.  8,192 × 8,192: 600 us, 920 TFLOP/s, causal
+// 870; over 4-bit pages 945 and 865 (a large f16 product of the library: 1,180).
 #include "lds_dma.h"
 #include "paged_dev.h"
 #include "wt.h"
@@ -80,7 +86,7 @@ __device__ __forceinline__ uint32_t lo16(uint32_t a, uint32_t b) { return __buil
 __device__ __forceinline__ uint32_t hi16(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
-// inclusive prefix sum over the wave, and its maximum (of values >= 0), on DPP: rows of 16 by shifts, then each row's last
+// inclusive prefix sum and prefix maximum (of values >= 0) over the wave, on DPP: rows of 16 by shifts, then each row's last
 // lane to the rows behind it
 template <int CTRL, int ROWS>
 __device__ __forceinline__ int dpp_or_0(int v) {
@@ -95,30 +101,36 @@ __device__ __forceinline__ int wave_scan(int v) {
     v += dpp_or_0<0x143, 0xc>(v);
     return v;
 }
-__device__ __forceinline__ int wave_top(int v) {
+__device__ __forceinline__ int wave_scan_max(int v) {
     v = max(v, dpp_or_0<0x111, 0xf>(v));
     v = max(v, dpp_or_0<0x112, 0xf>(v));
     v = max(v, dpp_or_0<0x114, 0xf>(v));
     v = max(v, dpp_or_0<0x118, 0xf>(v));
     v = max(v, dpp_or_0<0x142, 0xa>(v));
-    v = max(v, dpp_or_0<0x143, 0xc>(v));
-    return __builtin_amdgcn_readlane(v, 63);
+    return max(v, dpp_or_0<0x143, 0xc>(v));
 }
 
 // what one sequence asks for (per lane while scanning, uniform afterwards)
 struct SeqWork {
     int row0, nq, len, lo;   // first row of q, rows, keys, first key that any row sees
 };
+// that of sequence s0 + lane; `edge`: where the rows of sequence s0 begin, becomes where those of s0 + 64 do.  (Whatever
+// q_start holds, the sequences' rows lie side by side in [0, rows): the lists below cannot grow past what the host reckons)
 __device__ __forceinline__ SeqWork seq_work(const KvPages& c, const AttnArgs& a, const int* q_start, const int* kv_len,
-                                            int rows, int s) {
+                                            int rows, int s0, int lane, int& edge) {
     SeqWork w;
-    w.row0 = max(q_start[s], 0);
-    w.nq = max(min(q_start[s + 1], rows) - w.row0, 0);
-    w.len = (int)min((int64_t)max(kv_len[s], 0), (int64_t)c.max_pages << c.page_shift);
+    const int s = s0 + lane;
+    const bool is = s < c.n_seq;
+    const int end = max(wave_scan_max(is ? min(max(q_start[s + 1], 0), rows) : 0), edge);
+    w.row0 = __builtin_amdgcn_update_dpp(edge, end, 0x138, 0xf, 0xf, false);   // the lane before's
+    w.nq = end - w.row0;
+    edge = __builtin_amdgcn_readlane(end, 63);
+    w.len = is ? (int)min((int64_t)max(kv_len[s], 0), (int64_t)c.max_pages << c.page_shift) : 0;
     // the first row's window starts furthest left; with len < nq its position is negative
     w.lo = a.window > 0 ? max(w.len - w.nq - a.window + 1, 0) : 0;
     return w;
 }
+__device__ __forceinline__ int first_row(const int* q_start, int rows) { return uniform(min(max(q_start[0], 0), rows)); }
 
 // the registers of one wave's 32 keys
 template <int HD, int CT>
@@ -293,7 +305,12 @@ __device__ __forceinline__ void store_out(void* o, int o_type, int64_t at, f32x4
 // ------------------------------------------------------------------------------------------------ few rows
 // One launch over every sequence: the work is the list of (sequence, 16-row tile, KV head) items, each ⌈keys / 128⌉ tiles
 // long; workgroup w takes tiles [w · per, (w + 1) · per) of the whole list, so lengths that differ a thousandfold load the
-// workgroups alike.  A workgroup's part of an item is a segment; a segment that is not its whole item leaves its
+// workgroups alike.  No K/V byte passes LDS: K rows are loaded in the first operand's layout (v_mfma_f32_16x16x32: 16 keys ×
+// 16 rows), a lane loads hd/16 dims of its 8 keys of V and pairs them key by key in registers (v_perm), which makes MFMA row
+// m of tile t dim (hd/16) m + t; contraction slot (lane >> 4, j) stands for key 16 (j >> 2) + 4 (lane >> 4) + (j & 3), the
+// order in which the lane has its weights.  A wave's next K is loaded as soon as its scores are there, V behind its product
+// (two sets of registers instead: one workgroup less a CU, and spills).
+// A workgroup's part of an item is a segment; a segment that is not its whole item leaves its
 // (m, l, Oᵀ) in the scratch, and the last of the item's workgroups to arrive adds them up in their order (the result does
 // not depend on who is last).  Slot 0 of a workgroup: the item began in an earlier one; slot 1: it goes on in a later one.
 template <int HD, int CT, int QT>
@@ -322,16 +339,18 @@ __global__ __launch_bounds__(256, wgs_per_cu(HD, CT)) void k_paged_attn(KvPages 
     int chunk = 0, before = 0, total = 0;   // first sequence held in the lanes, tiles before it, all tiles
     SeqWork my{};
     int scan = 0;   // tiles up to and with this lane's sequence, from `chunk` on
+    const int row_first = first_row(q_start, rows);
+    int edge = row_first;
     auto hold = [&](int s0) {
         chunk = s0;
-        my = SeqWork{0, 0, 0, 0};
-        if (s0 + lane < c.n_seq) my = seq_work(c, a, q_start, kv_len, rows, s0 + lane);
+        if (s0 == 0) edge = row_first;
+        my = seq_work(c, a, q_start, kv_len, rows, s0, lane, edge);
         scan = wave_scan(my.nq > 0 ? items_of(my) * tiles_of(my) : 0);
     };
     for (int s0 = 0; s0 < c.n_seq; s0 += LANES) {
         hold(s0);
         total += __builtin_amdgcn_readlane(scan, 63);
-        longest = max(longest, wave_top(my.nq > 0 ? tiles_of(my) : 0));
+        longest = max(longest, __builtin_amdgcn_readlane(wave_scan_max(my.nq > 0 ? tiles_of(my) : 0), 63));
     }
     // a long item in at most kPieces parts: their arrivals are counted one after the other, 40 to 80 ns each
     const int per = max((total + (int)gridDim.x - 1) / (int)gridDim.x, (longest + kPieces - 1) / kPieces);
@@ -692,6 +711,8 @@ __global__ __launch_bounds__(256, wgs_per_cu(HD, CT)) void k_paged_attn(KvPages 
 // Work: items (sequence, 128 rows, KV head), the longest first, KV heads side by side (neighbouring workgroups go to
 // different XCDs: with 8 heads an XCD's L2 serves one).  Where the items are too few for the chip, `splits` workgroups
 // share one item's keys and the last to arrive joins their parts.
+// (Tried, for two prompts of 4,097 and 3,512 rows on 8,192 and 6,001 keys, 424 us: 8 waves in two groups a phase apart, one
+// multiplying while the other takes its softmax, 550 us; the next tile's scores interleaved with the exponentials, 486 us.)
 constexpr int kRowBlock = 128, kPromptKeys = 64;
 constexpr int kPromptSlots = 1024;   // parts of all items together where items are split
 // parts of one item at most, and tiles of a part at least: the last to arrive reads the others' 64 KB each, about 1 us
@@ -727,10 +748,9 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_paged_prompt(
     const int kvh = item % c.nkv;
     int blk = item / c.nkv;   // row block, counted over the sequences
     SeqWork x{};
-    int seq = -1;
+    int seq = -1, edge = first_row(q_start, rows);
     for (int s0 = 0; s0 < c.n_seq; s0 += 64) {
-        SeqWork my{};
-        if (s0 + lane < c.n_seq) my = seq_work(c, a, q_start, kv_len, rows, s0 + lane);
+        const SeqWork my = seq_work(c, a, q_start, kv_len, rows, s0, lane, edge);
         const int blocks = (my.nq * G + kRowBlock - 1) / kRowBlock, scan = wave_scan(blocks);
         const int in = __builtin_amdgcn_readlane(scan, 63);
         if (blk < in) {
@@ -1147,10 +1167,13 @@ static void launch(const KvPages& c, const AttnArgs& a, const void* q, int64_t l
     const int o_vec = ldo % 4 == 0 && ((uintptr_t)o & 15) == 0;
     unsigned* cnt = (unsigned*)ws;
     float* part = (float*)((char*)ws + kSplitWgs * 4);
-    if (is_prompt(c, a)) {
+    const int64_t row_tiles = ((int64_t)rows * G / 16 + c.n_seq) * c.nkv;   // at most
+    // (a list of 2^30 tiles or more, from far more rows than announced, is the prompt kernel's too: unsplit, without scratch)
+    const bool prompt = is_prompt(c, a);
+    if (prompt || row_tiles * cdiv64(((int64_t)c.max_pages << c.page_shift) + 1, kTileKeys) >= 1 << 30) {
         const int64_t items = ((int64_t)rows * G / kRowBlock + c.n_seq) * c.nkv;   // at most
-        QASR_CHECK(items < 1 << 23, QASR_E_CAPACITY, "paged_attention: too many rows for one call");
-        const int splits = (int)std::min<int64_t>(kPromptParts, std::max<int64_t>(1, kPromptSlots / items));
+        QASR_CHECK(items < 1 << 24, QASR_E_CAPACITY, "paged_attention: too many rows for one call");
+        const int splits = prompt ? (int)std::min<int64_t>(kPromptParts, std::max<int64_t>(1, kPromptSlots / items)) : 1;
         const size_t lds = 4 * kPromptKeys * HD * 2;
         if constexpr (HD == 256)   // (for the current device; past 64 KB)
             QASR_HIP(hipFuncSetAttribute((const void*)k_paged_prompt<HD, CT, QT>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
@@ -1158,10 +1181,7 @@ static void launch(const KvPages& c, const AttnArgs& a, const void* q, int64_t l
                                                                                part, cnt, splits, q_vec, o_vec);
         return;
     }
-    const int64_t items = ((int64_t)rows * G / 16 + c.n_seq) * c.nkv;   // at most
-    QASR_CHECK(items * cdiv64(((int64_t)c.max_pages << c.page_shift) + 1, kTileKeys) < 1 << 30, QASR_E_CAPACITY,
-               "paged_attention: too many rows for the max_q that they were announced with");
-    const int64_t tiles = items * std::max<int64_t>(1, cdiv64(a.max_kv, kTileKeys));
+    const int64_t tiles = row_tiles * std::max<int64_t>(1, cdiv64(a.max_kv, kTileKeys));
     const int grid = (int)std::min<int64_t>(256 * wgs_per_cu(HD, CT), tiles);
     k_paged_attn<HD, CT, QT><<<grid, 256, 0, s>>>(c, a, q, ldq, q_start, kv_len, rows, o, ldo, part, cnt, q_vec,
                                                   o_vec);

@@ -88,9 +88,9 @@ def attend(q, k, v, q_start, kv_len, table, scale, causal, window, out):
     weighted mean and the plain sum of |v| that the tolerances go by."""
     nh, nkv, page, n_pages = q.shape[1], k.shape[1], k.shape[2], k.shape[0]
     mag, total = np.zeros_like(out), np.zeros_like(out)
+    edge = np.maximum.accumulate(np.clip(q_start, 0, len(q)))     # rows of sequences lie side by side
     for s in range(len(kv_len)):
-        r0, r1 = max(0, q_start[s]), min(len(q), q_start[s + 1])
-        n = r1 - r0
+        r0, n = edge[s], edge[s + 1] - edge[s]
         length = min(max(0, kv_len[s]), table.shape[1] * page)
         pos = np.arange(length)
         ids = table[s][pos // page]

@@ -123,7 +123,7 @@ def test_attention_arguments_refused():
         refused(lib.qasr_op_paged_attention(*ok[:at], bad, *ok[at + 1:]))
     _lib.check(lib.qasr_paged_attention_workspace(C.byref(cache()), C.byref(attn()), C.byref(n)))
     if n.value:
-        for ws, size in ((None, n.value), (A, n.value - 1), (A + 8, n.value)):
+        for ws, size in ((None, n.value), (A, n.value - 1), (A + 8, n.value), (A + 64, n.value)):
             refused(lib.qasr_op_paged_attention(*ok[:9], ws, size, None), 6)
     _lib.check(lib.qasr_op_paged_attention(C.byref(cache()), C.byref(attn()), None, 512, None, None, 0, None, 512, None,
                                            0, None))

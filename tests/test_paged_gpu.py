@@ -109,6 +109,24 @@ def test_rope_padding_rows_and_in_place(torch_dev):
             assert np.array_equal(got[i], x_h[i].astype(np.float64))
 
 
+@pytest.mark.parametrize("rows,heads,hd,rot,inter", [(700, 7, 128, 128, False), (700, 7, 128, 64, True),
+                                                     (9, 3, 80, 20, False), (1500, 16, 256, 128, False)])
+def test_rope_in_place_many_rows(torch_dev, rows, heads, hd, rot, inter):
+    """in place gives what a second buffer gets, bit for bit, in every form of the kernel"""
+    import torch
+
+    rng = np.random.default_rng(rows + rot)
+    x = dev(rng.standard_normal((rows, heads * hd)).astype(np.float32), "bf16")
+    cs, w = dev(table(rows, rot)), dev(1 + 0.2 * rng.standard_normal(hd).astype(np.float32))
+    pos, y = dev(rng.permutation(rows).astype(np.int32)), torch.empty_like(x)
+    r = rope_args(cs, rot, inter, w)
+    for out in (y, x):
+        _lib.check(_lib.load().qasr_op_rope(x.data_ptr(), 2, heads * hd, pos.data_ptr(), rows, heads, hd, C.byref(r),
+                                            out.data_ptr(), 2, heads * hd, stream()))
+    torch.cuda.synchronize()
+    assert torch.equal(x, y)
+
+
 @pytest.mark.parametrize("rot", [2, 20, 64, 128])
 @pytest.mark.parametrize("kind", [0, 1, 2, 3])
 @pytest.mark.parametrize("first,n", [(0, 1), (0, 700), (131072 - 65, 65), ((1 << 40) - 3, 4), (5, 0)])
@@ -455,9 +473,38 @@ def test_attention_bad_entries(torch_dev, kv, qt):
     c.table = dev(c.table_h)
     o = attend(c, q, qs, kl, 2, True, 0, 0.1)
     check_attend(c, q, o, qs, kl, 2, True, 0, 0.1, qt, qt)
-    for qs2, kl2 in (([0, 1, 21, 30], [10 ** 9, -7, 64]), ([-3, 1, 1, 24], [20, 3, 64]), ([5, 3, 10, 12], [20, 50, 1])):
-        o = attend(c, q, qs2, kl2, 2, True, 0, 0.1, max_q=30, max_kv=100)
-        check_attend(c, q, o, qs2, kl2, 2, True, 0, 0.1, qt, qt)
+    for qs2, kl2 in (([0, 1, 21, 30], [10 ** 9, -7, 64]), ([-3, 1, 1, 24], [20, 3, 64]), ([5, 3, 10, 12], [20, 50, 1]),
+                     ([20, 0, 20, 0], [20, 50, 1]), ([7, 2 ** 31 - 1, -2 ** 31, 9], [20, 50, 1])):
+        for max_q in (30, 1000):
+            o = attend(c, q, qs2, kl2, 2, True, 0, 0.1, max_q=max_q, max_kv=100)
+            check_attend(c, q, o, qs2, kl2, 2, True, 0, 0.1, qt, qt)
+
+
+@pytest.mark.parametrize("kv,qt", LAYOUTS)
+def test_attention_no_pages_and_odd_rows(torch_dev, kv, qt):
+    """a cache without pages gives zeros; a row of q that is no number stays the only one"""
+    import torch
+
+    rng = np.random.default_rng(18)
+    c, q, qs, kl = make(rng, kv, 16, 2, 2, 128, [90, 40], [37, 1], qt)
+    want = [num(attend(c, q, qs, kl, 4, True, 0, 0.1, max_q=m)) for m in (1, 1000)]
+    q[5, 128:256] = float("nan")
+    q[20, 300] = float("inf")
+    for m, was in zip((1, 1000), want):
+        got = num(attend(c, q, qs, kl, 4, True, 0, 0.1, max_q=m)).reshape(38, 4, 128)
+        was = was.reshape(38, 4, 128)
+        assert np.isnan(got[5, 1]).all()
+        same = np.ones((38, 4), bool)
+        same[5, 1] = same[20, 2] = False
+        assert np.array_equal(got[same], was[same])
+    d = c.desc()
+    for kw in (dict(n_pages=0, k=None, v=None), dict(max_pages=0, page_table=None)):
+        for name, value in kw.items():
+            setattr(d, name, value)
+        c.desc = lambda: d
+        for m in (1, 1000):
+            o = attend(c, q, qs, kl, 4, True, 0, 0.1, max_q=m)
+            assert (num(o) == 0).all()
 
 
 @pytest.mark.parametrize("kv,qt", LAYOUTS)
