@@ -715,8 +715,7 @@ __global__ __launch_bounds__(256, wgs_per_cu(HD, CT)) void k_paged_attn(KvPages 
 // multiplying while the other takes its softmax, 550 us; the next tile's scores interleaved with the exponentials, 486 us.)
 constexpr int kRowBlock = 128, kPromptKeys = 64;
 constexpr int kPromptSlots = 1024;   // parts of all items together where items are split
-// parts of one item at most, and tiles of a part at least: the last to arrive reads the others' 64 KB each, about 1 us
-constexpr int kPromptParts = 32, kPartTiles = 8;
+constexpr int kPromptParts = 32;     // … and of one item
 
 template <int HD>
 __device__ __forceinline__ int k_swz(int row) { return row & (HD / 8 - 1); }
@@ -729,6 +728,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_paged_prompt(
     const int* __restrict__ kv_len, int rows, void* __restrict__ o, int64_t ldo, float* part, unsigned* cnt, int splits,
     int q_vec, int o_vec) {
     constexpr int KK = HD / 16, DT = HD / 32, CPR = HD / 8, ROW = HD * 2;
+    constexpr bool kAhead = CT == T_MXFP4 || HD == 256;
     constexpr int kSlot = kRowBlock * (HD + 2);   // floats: Oᵀ as [wave][dim tile · 4 + i / 4][lane][4], then m, l per row
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     __shared__ int s_ok[2][4];
@@ -773,7 +773,10 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_paged_prompt(
     const int blk_hi = a.causal ? max(0, min(x.len, p0 + row_base / G + 1)) : x.len;
     const int blk_lo = a.window > 0 ? max(0, p0 + (row_base + nrow - 1) / G - a.window + 1) : 0;
     const int tile0 = b_lo / kPromptKeys, tiles = max(0, (b_hi + kPromptKeys - 1) / kPromptKeys - tile0);
-    const int parts = max(1, min(splits, tiles / kPartTiles));
+    // about what takes least: a part walks tiles / parts of 2.6 us and the join reads `parts` of about 1 us, one by one; and
+    // no more than fill the chip once (`splits` is for kPromptSlots workgroups), or twice with long parts, which end together
+    const int fill = max(splits / (HD == 256 ? 3 : 2), min(splits, tiles / 32));
+    const int parts = max(1, min((int)sqrtf(2.5f * tiles), fill));
     if (split >= parts) return;
     const int t_begin = tile0 + (int)((int64_t)tiles * split / parts), t_end = tile0 + (int)((int64_t)tiles * (split + 1) / parts);
 
@@ -944,14 +947,14 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_paged_prompt(
             for (int u = 0; u < 2; u++)
 #pragma unroll
                 for (int j = 0; j < 16; j++) sv[u][j] = 0.f;
-            // 4-bit pages: the operands of 8 steps are read ahead and each register's next one behind the product that frees
-            // it (prompts 3 % faster; over 16-bit pages, which do not hold the next tile in registers, 4 % slower)
-            constexpr int AHEAD = CT == T_MXFP4 ? (KK < 8 ? KK : 8) : 1, STEPS = 2 * KK;
+            // 4-bit pages, and one wave a SIMD: the operands of 8 steps are read ahead and each register's next one behind the
+            // product that frees it (4-bit pages 3 % faster; 16-bit ones of head_dim 128 4 % slower, two waves hide as much)
+            constexpr int AHEAD = kAhead ? (KK < 8 ? KK : 8) : 1, STEPS = 2 * KK;
             auto read_k = [&](int i) {   // step i: half i / KK, dims 16 (i % KK) ..
                 const int row = 32 * (i / KK) + n, ch = 2 * (i % KK) + h;
                 return *(const u32x4*)(ldsK + buf * TILE + row * ROW + 16 * (ch ^ k_swz<HD>(row)));
             };
-            if constexpr (CT == T_MXFP4) {
+            if constexpr (kAhead) {
                 u32x4 kf[AHEAD];
 #pragma unroll
                 for (int i = 0; i < AHEAD; i++) kf[i] = read_k(i);
@@ -1046,7 +1049,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_paged_prompt(
         }
         __builtin_amdgcn_s_setprio(1);
         if (active) {
-            if constexpr (CT == T_MXFP4) {
+            if constexpr (kAhead) {
                 u32x4 vf[DT];
 #pragma unroll
                 for (int dt = 0; dt < DT; dt++) vf[dt] = read_v(buf, 0, 0, dt);
