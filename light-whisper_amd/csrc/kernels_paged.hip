@@ -9,7 +9,8 @@ namespace qasr {
 // ------------------------------------------------------------------------------------------------ table
 // A thread takes one frequency and `run` positions: the angle's sine and cosine once, in 64 bits, and from there each next
 // position by one rotation (4 multiply-adds in 64 bits; after 32 of them off by 2^-48 at most, the result is rounded to
-// 24 bits).  Bound by the stores: neighbouring lanes hold neighbouring frequencies.
+// 24 bits).  Bound by the stores: neighbouring lanes hold neighbouring frequencies.  131,072 positions of 64: 67 MB in 13 us,
+// 5.1 TB/s (an angle's own sine for each: 40 us).
 __global__ __launch_bounds__(256) void k_rope_table(RopeFreqs f, int64_t first, int n_pos, int run, float2* __restrict__ cs) {
     const int half = f.rot / 2;
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, p0 = i / half * run;
@@ -91,8 +92,8 @@ __device__ void head_to_lds(const void* x, int64_t off, int hd, const RopeArgs& 
 // the half layout (each pair in one thread), 8 u and hd/2 + 8 u in the interleaved one, and the two halves of the dims that
 // do not rotate likewise.  The head's hd / 16 threads are neighbours, so a run of lanes reads a run of bytes (a lane's 16
 // dims in one piece: a third slower) and the norm's sum is a few xor-shuffles.  A thread takes up to four heads of its row
-// with one read of the table.  Bound by memory.
-constexpr int kHeadsPer = 4;
+// with one read of the table.  Bound by memory: 8,192 rows of 16 heads, bf16, half of each turned, 69 MB in 18 us (3.8 TB/s;
+// a copy of 2 GiB runs at 4.8).
 
 // 8 elements as they were loaded; they are widened only when they are used, so that many loads are in flight
 template <int T>
@@ -293,13 +294,16 @@ void rope_rows(const Rows& x, const int* pos, int rows, int heads, int hd, const
             constexpr int XT = xt(), YT = yt();
             if (units_ok(hd, r) && rows16(x) && rows16(y)) {
                 const int ll = log2_up(hd / 16);
-                // few rows: a head a thread group, so that more of the chip works on them; many: four
+                // a head a thread while all of them fit the chip at once (900 x 16 heads, f32: 5.6 against 7.0 us with four);
+                // past that, as many heads as 64 registers hold of x (8,192 x 16: f32 two, 28 us, one or four 30; f16 four,
+                // 18 us, one 20)
+                constexpr int HP = XT == T_F32 ? 2 : 4;
                 const int64_t all = (int64_t)rows * heads;
-                if (all << ll < 65536)
+                if (all << ll < 8 * 65536)
                     k_rope_units<XT, YT, 1><<<unit_grid(all, ll), 256, 0, s>>>(x.p, x.ld, pos, rows, heads, hd, ll, r,
                                                                                (void*)y.p, y.ld);
                 else
-                    k_rope_units<XT, YT, kHeadsPer><<<unit_grid((int64_t)rows * cdiv(heads, kHeadsPer), ll), 256, 0, s>>>(
+                    k_rope_units<XT, YT, HP><<<unit_grid((int64_t)rows * cdiv(heads, HP), ll), 256, 0, s>>>(
                         x.p, x.ld, pos, rows, heads, hd, ll, r, (void*)y.p, y.ld);
             } else {
                 k_rope_any<XT, YT><<<(unsigned)std::min<int64_t>((int64_t)rows * heads, 1 << 20), 64, 0, s>>>(
@@ -351,7 +355,9 @@ __device__ __forceinline__ void fp4_put(uint8_t* blk, uint32_t codes, int hd, in
 }
 
 // a thread: 16 dims of K (even waves) or V (odd ones) of one KV head, as k_rope_units; hd is a power of two, so every thread
-// has dims.  (K and V in one thread: with K in 64 bits, 154 registers, a third of the waves and a third more time)
+// has dims.  f32 rows of 8 heads into bf16 pages: 8,191 rows, 101 MB in 23.5 us (4.3 TB/s).  Into 4-bit pages 37 us for 76 MB:
+// there the 64-bit arithmetic of K (below) takes the registers that would hide its loads (in 32 bits 27 us; 32 bits with
+// 64 only next to a border 36, the rare branch takes the same registers; fewer registers by force spill: 67 and more)
 template <int XT, int CT>
 __global__ __launch_bounds__(256) void k_kv_append_units(KvPages c, const void* k, const void* v, int64_t ldk, int64_t ldv,
                                                          const int* __restrict__ seq, const int* __restrict__ pos, int rows,
@@ -476,7 +482,7 @@ __device__ __forceinline__ void block_values(const KvPages& c, const uint8_t* bl
     }
 }
 
-// a thread: 8 dims of K and of V of one KV head
+// a thread: 8 dims of K and of V of one KV head.  8,191 rows of 8 heads from 4-bit pages to f32: 76 MB in 18 us (4.2 TB/s)
 template <int CT, int YT, bool WIDE>
 __global__ __launch_bounds__(256) void k_kv_gather(KvPages c, const int* __restrict__ seq, const int* __restrict__ pos,
                                                    int rows, void* k, void* v, int64_t ldk, int64_t ldv) {
