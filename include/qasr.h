@@ -447,7 +447,8 @@ typedef struct {
                               (more are computed all the same, more slowly) */
 } qasr_paged_attn;
 /* Bytes of scratch (128-byte aligned) for calls with these descriptions; zero it once, every call leaves it ready for the
-   next.  A scratch serves one call at a time: calls (or graphs) that may overlap need one each. */
+   next.  One as large as the largest serves calls of several descriptions, one after the other: calls (or graphs) that may
+   overlap need one each. */
 QASR_API int qasr_paged_attention_workspace(const qasr_kv_cache* c, const qasr_paged_attn* a, size_t* bytes);
 QASR_API int qasr_op_paged_attention(const qasr_kv_cache* c, const qasr_paged_attn* a, const void* q, int64_t ldq,
                                      const int32_t* q_start /* [n_seq + 1] */, const int32_t* kv_len /* [n_seq] */,

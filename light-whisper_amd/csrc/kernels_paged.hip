@@ -355,7 +355,7 @@ __device__ __forceinline__ void fp4_put(uint8_t* blk, uint32_t codes, int hd, in
 }
 
 // a thread: 16 dims of K (even waves) or V (odd ones) of one KV head, as k_rope_units; hd is a power of two, so every thread
-// has dims.  f32 rows of 8 heads into bf16 pages: 8,191 rows, 101 MB in 23.5 us (4.3 TB/s).  Into 4-bit pages 37 us for 76 MB:
+// has dims.  f32 rows of 8 heads into bf16 pages: 8,191 rows, 101 MB in 23.5 us (4.3 TB/s).  Into 4-bit pages 39 us for 76 MB:
 // there the 64-bit arithmetic of K (below) takes the registers that would hide its loads (in 32 bits 27 us; 32 bits with
 // 64 only next to a border 36, the rare branch takes the same registers; fewer registers by force spill: 67 and more)
 template <int XT, int CT>

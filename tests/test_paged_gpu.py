@@ -701,3 +701,45 @@ def test_graph_replays_and_streams(torch_dev, kv):
         check_attend(c, bufs[2][0], bufs[2][1], qs.cpu().numpy(), kl.cpu().numpy(), nh, True, 0, 0.09, "f16", "f16")
         pos.add_(1)
         kl.add_(1)
+
+
+@pytest.mark.parametrize("kv,qt", LAYOUTS)
+@pytest.mark.parametrize("hd", [64, 256])
+def test_one_workspace_for_prompts_and_tokens(torch_dev, kv, qt, hd):
+    """a captured prompt whose keys are shared out between workgroups, then single tokens, alternating on one workspace:
+    each replay gives what an eager call on a fresh one does, and the workspace's counters end as they began"""
+    import torch
+
+    nkv, g, page = 2, 2, 32
+    nh, scale = nkv * g, hd ** -0.5
+    rng = np.random.default_rng(hd)
+    lens = [2900, 4100]
+    c, q, qs, kl = make(rng, kv, page, nkv, g, hd, lens, [150, 70], qt)
+    lib, d, size = _lib.load(), c.desc(), C.c_size_t()
+    a = [_lib.PagedAttn(n_heads=nh, q_type=IDS[qt], o_type=IDS[qt], causal=1, window=0, scale=scale, max_q=m, max_kv=4100)
+         for m in (150, 1)]
+    most = 0
+    for x in a:
+        _lib.check(lib.qasr_paged_attention_workspace(C.byref(d), C.byref(x), C.byref(size)))
+        most = max(most, size.value)
+    ws = torch.zeros(most, dtype=torch.uint8, device="cuda:0")
+    starts, klen = [dev(qs), dev(np.arange(3, dtype=np.int32))], dev(kl)
+    outs = [torch.empty((n, nh * hd), dtype=T(qt), device="cuda:0") for n in (220, 2)]
+    g_ = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g_):
+        for x, st, o in zip(a, starts, outs):
+            _lib.check(lib.qasr_op_paged_attention(C.byref(d), C.byref(x), q.data_ptr(), nh * hd, st.data_ptr(),
+                                                   klen.data_ptr(), o.shape[0], o.data_ptr(), nh * hd, ws.data_ptr(),
+                                                   most, torch.cuda.current_stream().cuda_stream))
+    for i in range(4):
+        for o in outs:
+            o.fill_(9.0)
+        torch.cuda.synchronize()
+        g_.replay()
+        torch.cuda.synchronize()
+        want = [attend(c, q, qs, kl, nh, True, 0, scale), attend(c, q[:2], [0, 1, 2], kl, nh, True, 0, scale)]
+        assert all(torch.equal(x, y) for x, y in zip(outs, want))
+        check_attend(c, q, outs[0], qs, kl, nh, True, 0, scale, qt, qt)
+        check_attend(c, q[:2], outs[1], [0, 1, 2], kl, nh, True, 0, scale, qt, qt)
+        q.copy_(dev(rng.standard_normal(tuple(q.shape)).astype(np.float32), qt))
+    assert int(ws[:4096].sum()) == 0
