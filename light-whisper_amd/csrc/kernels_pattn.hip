@@ -717,6 +717,14 @@ constexpr int kRowBlock = 128, kPromptKeys = 64;
 constexpr int kPromptSlots = 1024;   // parts of all items together where items are split
 constexpr int kPromptParts = 32;     // … and of one item
 
+// Parts of an item of so many tiles.  About what takes least: a part walks tiles / parts of 2.6 us and the join reads `parts`
+// of about 1 us, one by one, and a few us to be there at all (2 tiles: 14.8 us alone, 16.0 in two parts); and no more than fill
+// the chip once (`fill` parts of every item are kPromptSlots), or twice with long parts, which end together
+__host__ __device__ inline int prompt_parts(int tiles, int fill, int hd, int most) {
+    const int n = max(fill / (hd == 256 ? 3 : 2), min(fill, tiles / 32));
+    return tiles < 6 ? 1 : max(1, min(min((int)sqrtf(2.5f * tiles), n), most));
+}
+
 template <int HD>
 __device__ __forceinline__ int k_swz(int row) { return row & (HD / 8 - 1); }
 template <int HD>
@@ -726,7 +734,7 @@ template <int HD, int CT, int QT>
 __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_paged_prompt(
     KvPages c, AttnArgs a, const void* __restrict__ q, int64_t ldq, const int* __restrict__ q_start,
     const int* __restrict__ kv_len, int rows, void* __restrict__ o, int64_t ldo, float* part, unsigned* cnt, int splits,
-    int q_vec, int o_vec) {
+    int fill, int q_vec, int o_vec) {
     constexpr int KK = HD / 16, DT = HD / 32, CPR = HD / 8, ROW = HD * 2;
     constexpr bool kAhead = CT == T_MXFP4 || HD == 256;
     constexpr int kSlot = kRowBlock * (HD + 2);   // floats: Oᵀ as [wave][dim tile · 4 + i / 4][lane][4], then m, l per row
@@ -773,10 +781,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_paged_prompt(
     const int blk_hi = a.causal ? max(0, min(x.len, p0 + row_base / G + 1)) : x.len;
     const int blk_lo = a.window > 0 ? max(0, p0 + (row_base + nrow - 1) / G - a.window + 1) : 0;
     const int tile0 = b_lo / kPromptKeys, tiles = max(0, (b_hi + kPromptKeys - 1) / kPromptKeys - tile0);
-    // about what takes least: a part walks tiles / parts of 2.6 us and the join reads `parts` of about 1 us, one by one; and
-    // no more than fill the chip once (`splits` is for kPromptSlots workgroups), or twice with long parts, which end together
-    const int fill = max(splits / (HD == 256 ? 3 : 2), min(splits, tiles / 32));
-    const int parts = max(1, min((int)sqrtf(2.5f * tiles), fill));
+    const int parts = prompt_parts(tiles, fill, HD, splits);
     if (split >= parts) return;
     const int t_begin = tile0 + (int)((int64_t)tiles * split / parts), t_end = tile0 + (int)((int64_t)tiles * (split + 1) / parts);
 
@@ -1148,18 +1153,28 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_paged_prompt(
 }  // namespace
 
 // Which kernel, by the rows (tokens · heads of a KV head) of a sequence.  The few-row one reads the keys anew for every 16
-// rows, which L2 bears for a while; the prompt one has whole blocks of 128 rows to fill and more to start.  Measured (f16,
-// one sequence of 32,768 keys, 16 / 8 heads): 64 rows 58 against 64 us, 128 rows 90 against 66; over 4-bit pages, a quarter of
-// the bytes, 256 rows 105 against 89 us (32 x 4,096 keys: 93 against 100); 2,000 keys: 256 rows 20 against 36 us
-static bool is_prompt(const KvPages& c, const AttnArgs& a) {
-    const int64_t few = c.type == T_MXFP4 || a.max_kv <= 2048 ? 256 : 64;
-    return (int64_t)a.max_q * (a.nh / c.nkv) > few;
+// rows, which L2 bears for a while; the prompt one has whole blocks of 128 rows to fill and more to start.  To 64 rows the
+// first (one sequence of 32,768 keys, 64 rows, 16 / 8 heads, f16: 58 against 64 us), past 256 the second; between them, over
+// 16-bit pages the first while its list gives no workgroup more than 5 tiles (f16, 256 rows: one sequence of 2,000 keys 20
+// against 25 us, of 8,192 46 against 40; 4 of 2,000 66 against 30; 16 of 2,000 102 against 46), over 4-bit ones up to 16,384
+// keys (256 rows: 64 x 2,000 keys 67 against 108 us, 16 x 8,192 127 against 124, 4 x 32,768 284 against 199)
+enum Rule { kFew, kMid, kMany };
+static Rule rule_of(const KvPages& c, const AttnArgs& a) {
+    const int64_t r = (int64_t)a.max_q * (a.nh / c.nkv);
+    return r <= 64 ? kFew : r <= 256 ? kMid : kMany;
+}
+static bool is_prompt(const KvPages& c, const AttnArgs& a, int64_t row_tiles) {
+    const Rule rule = rule_of(c, a);
+    if (rule != kMid) return rule == kMany;
+    const int64_t keys = a.window > 0 ? std::min((int64_t)a.max_kv, (int64_t)a.window + a.max_q) : a.max_kv;
+    if (c.type == T_MXFP4) return keys > 16384;
+    return row_tiles * cdiv64(keys, kTileKeys) > 5 * 256 * wgs_per_cu(c.hd, c.type);
 }
 
 size_t paged_attention_ws(const KvPages& c, const AttnArgs& a) {
     const size_t few = (size_t)kSplitWgs * 4 + (size_t)kSplitWgs * 2 * (16 * c.hd + 32) * 4;
     const size_t many = (size_t)kSplitWgs * 4 + (size_t)kPromptSlots * kRowBlock * (c.hd + 2) * 4;
-    return is_prompt(c, a) ? many : few;
+    return rule_of(c, a) == kFew ? few : std::max(few, many);
 }
 
 template <int HD, int CT, int QT>
@@ -1170,18 +1185,25 @@ static void launch(const KvPages& c, const AttnArgs& a, const void* q, int64_t l
     const int o_vec = ldo % 4 == 0 && ((uintptr_t)o & 15) == 0;
     unsigned* cnt = (unsigned*)ws;
     float* part = (float*)((char*)ws + kSplitWgs * 4);
-    const int64_t row_tiles = ((int64_t)rows * G / 16 + c.n_seq) * c.nkv;   // at most
+    const int used = std::min(rows, c.n_seq);   // sequences with rows, at most
+    const int64_t row_tiles = ((int64_t)rows * G / 16 + used) * c.nkv;
     // (a list of 2^30 tiles or more, from far more rows than announced, is the prompt kernel's too: unsplit, without scratch)
-    const bool prompt = is_prompt(c, a);
+    const bool prompt = is_prompt(c, a, row_tiles);
     if (prompt || row_tiles * cdiv64(((int64_t)c.max_pages << c.page_shift) + 1, kTileKeys) >= 1 << 30) {
-        const int64_t items = ((int64_t)rows * G / kRowBlock + c.n_seq) * c.nkv;   // at most
+        const int64_t items = ((int64_t)rows * G / kRowBlock + used) * c.nkv;   // at most
         QASR_CHECK(items < 1 << 24, QASR_E_CAPACITY, "paged_attention: too many rows for one call");
-        const int splits = prompt ? (int)std::min<int64_t>(kPromptParts, std::max<int64_t>(1, kPromptSlots / items)) : 1;
+        const int fill = (int)std::min<int64_t>(kPromptParts, std::max<int64_t>(1, kPromptSlots / items));
+        // the most parts that an item as long as announced is cut into: a workgroup without one holds a place until it has
+        // found that out (3 x 308 rows of 5 heads of 256 on up to 5,339 keys: 52 us, with all `fill` launched 116; with a
+        // window of 100 keys 22 against 87)
+        int64_t keys = std::min<int64_t>(a.max_kv, 1 << 30);
+        if (a.window > 0) keys = std::min<int64_t>(keys, (int64_t)a.window + kPromptKeys + (a.causal ? kRowBlock / G : a.max_q));
+        const int splits = prompt ? prompt_parts((int)cdiv64(keys, kPromptKeys) + 1, fill, HD, fill) : 1;
         const size_t lds = 4 * kPromptKeys * HD * 2;
         if constexpr (HD == 256)   // (for the current device; past 64 KB)
             QASR_HIP(hipFuncSetAttribute((const void*)k_paged_prompt<HD, CT, QT>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
         k_paged_prompt<HD, CT, QT><<<(unsigned)(items * splits), 256, lds, s>>>(c, a, q, ldq, q_start, kv_len, rows, o, ldo,
-                                                                               part, cnt, splits, q_vec, o_vec);
+                                                                               part, cnt, splits, fill, q_vec, o_vec);
         return;
     }
     const int64_t tiles = row_tiles * std::max<int64_t>(1, cdiv64(a.max_kv, kTileKeys));

@@ -743,3 +743,17 @@ def test_one_workspace_for_prompts_and_tokens(torch_dev, kv, qt, hd):
         check_attend(c, q[:2], outs[1], [0, 1, 2], kl, nh, True, 0, scale, qt, qt)
         q.copy_(dev(rng.standard_normal(tuple(q.shape)).astype(np.float32), qt))
     assert int(ws[:4096].sum()) == 0
+
+
+@pytest.mark.parametrize("kv,qt", LAYOUTS)
+@pytest.mark.parametrize("nq,lens,window,max_kv,max_q", [
+    ([70, 1, 128], [900, 3000, 2100], 0, None, None), ([70, 1, 128], [900, 3000, 2100], 100, None, None),
+    ([300, 17], [2600, 30], 64, None, None), ([300, 17], [2600, 1900], 0, 1, None), ([200], [5000], 0, 64, None),
+    ([128] * 6, [700] * 6, 0, None, None), ([65, 65], [17000, 100], 0, None, None), ([400], [3000], 300, None, 40),
+    ([100, 0, 90], [6000, 9, 90], 5900, 1 << 30, 1 << 20)])
+def test_attention_split_choices(torch_dev, kv, qt, nq, lens, window, max_kv, max_q):
+    """every way in which rows, keys, windows and what was announced of them share a call out"""
+    rng = np.random.default_rng(sum(nq) + window)
+    c, q, qs, kl = make(rng, kv, 64, 2, 2, 128, lens, nq, qt)
+    o = attend(c, q, qs, kl, 4, True, window, 0.09, max_kv=max_kv, max_q=max_q)
+    check_attend(c, q, o, qs, kl, 4, True, window, 0.09, qt, qt)
