@@ -5,7 +5,7 @@
 //   Sᵀ = K·Qᵀ   (keys × rows; a lane holds scores of ONE row, so the softmax needs no cross-lane work but a vote)
 //   Oᵀ = Vᵀ·Pᵀ  (dims × rows; a lane's weights are the second operand as they stand, V is brought to match)
 // One pass over the keys with a running maximum that moves only where some row's rises by more than 2^kSlack: weights are
-// exp2(s − m + kUp), sums and Oᵀ in f32.  Roundings: the weights to q's type for the product with V (half a step each; f16
+// exp2(s − m + lift), sums and Oᵀ in f32.  Roundings: the weights to q's type for the product with V (half a step each; f16
 // reaches 2^-26 of the largest before its steps stop shrinking), the output to its type.  e2m1 · 2^E is exact in either type.
 //
 // Few rows (k_paged_attn): bound by memory.  16 / 8 heads of 128, f16: one sequence of 32,768 keys 32 us (134 MB, 4.1 TB/s),
@@ -35,9 +35,16 @@ constexpr int kTileKeys = 128;   // keys of one workgroup step: 32 for each of i
 constexpr int kSplitWgs = 1024;  // workgroups at most (what the scratch is sized for)
 // workgroups that a CU holds by their registers
 constexpr int wgs_per_cu(int hd, int ct) { return ct == T_MXFP4 ? (hd == 256 ? 2 : 3) : hd == 256 ? 1 : 2; }
-// weights are exp2(s − m + kUp), m at most kSlack below the running maximum: at most 2^15 in f16, and its normal range
-// reaches 26 bits further down
+// weights are exp2(s − m + lift), m at most kSlack below the running maximum.  f16 and 4-bit pages: lift = kUp, weights of at
+// most 2^15 in f16, whose normal range reaches 26 bits further down, and V of at most 2^16 leaves the sums far below f32's
+// largest.  bf16 pages hold V up to that: there a row's weights, one for each of its sequence's keys, sum to at most 1, so that
+// no partial sum of the product with V passes the largest |V| (at the other end, over 32,768 keys, V below 2^-108 meets f32's
+// smallest normal numbers)
 constexpr float kSlack = 3.f, kUp = 12.f;
+template <int CT>
+__device__ __forceinline__ float lift(int keys) {
+    return CT == T_BF16 ? -kSlack - (float)(32 - __clz(max(keys, 1) - 1)) : kUp;   // (bits of keys − 1: ⌈log2 keys⌉)
+}
 constexpr float kNone = -3.0e38f;   // running maximum before the first key
 
 template <int QT>
@@ -544,7 +551,7 @@ __global__ __launch_bounds__(256, wgs_per_cu(HD, CT)) void k_paged_attn(KvPages 
                     for (int t2 = 0; t2 < ND; t2++) acc[t2] *= al;
                 }
                 u32x4 pf;
-                const float mk = kUp - m;
+                const float mk = lift<CT>(x.len) - m;
 #pragma unroll
                 for (int j = 0; j < 8; j++) p[j] = __builtin_amdgcn_exp2f(fmaf(p[j], sc, mk));
 #pragma unroll
@@ -1005,7 +1012,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_paged_prompt(
 #pragma unroll
                 for (int i = 0; i < DT; i++) acc[i] *= al;
             }
-            const float mk = kUp - m;
+            const float mk = lift<CT>(x.len) - m;
 #pragma unroll
             for (int u = 0; u < 2; u++) {
                 float ls = 0.f;
