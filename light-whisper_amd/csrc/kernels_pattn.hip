@@ -45,7 +45,12 @@ template <int CT>
 __device__ __forceinline__ float lift(int keys) {
     return CT == T_BF16 ? -kSlack - (float)(32 - __clz(max(keys, 1) - 1)) : kUp;   // (bits of keys − 1: ⌈log2 keys⌉)
 }
-constexpr float kNone = -3.0e38f;   // running maximum before the first key
+constexpr float kNone = -3.40282347e38f;   // running maximum before the first key: no score is less
+// exp2(s · c + (lift − m)) is one multiply-add and one rounding of m, which is more than the slack in a weight's range once m
+// has 24 bits before the point: where a row's |m| is past kBig (a rounding of 2^-12), s · c − m is taken first, from the product
+// as m was, so that the largest gives 0 and none a larger weight than the lift and the slack allow
+constexpr float kBig = 4096.f;
+__device__ __forceinline__ bool is_big(float m) { return fabsf(m) > kBig && m != kNone; }
 
 template <int QT>
 __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
@@ -437,11 +442,13 @@ __global__ __launch_bounds__(256, wgs_per_cu(HD, CT)) void k_paged_attn(KvPages 
 
         f32x4 acc[ND];
         float m, l;
+        bool big = false;   // some row's m is
         auto clear = [&] {
 #pragma unroll
             for (int i = 0; i < ND; i++) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
             m = kNone;
             l = 0.f;
+            big = false;
         };
         clear();
 
@@ -547,13 +554,20 @@ __global__ __launch_bounds__(256, wgs_per_cu(HD, CT)) void k_paged_attn(KvPages 
                     const float mn = fmaxf(m, mx), al = __builtin_amdgcn_exp2f(m - mn);
                     m = mn;
                     l *= al;
+                    big = __any(is_big(m));
 #pragma unroll
                     for (int t2 = 0; t2 < ND; t2++) acc[t2] *= al;
                 }
                 u32x4 pf;
-                const float mk = lift<CT>(x.len) - m;
+                float c2 = sc, mk = lift<CT>(x.len) - m;
+                if (__builtin_expect(big, 0) && is_big(m)) {
 #pragma unroll
-                for (int j = 0; j < 8; j++) p[j] = __builtin_amdgcn_exp2f(fmaf(p[j], sc, mk));
+                    for (int j = 0; j < 8; j++) p[j] = p[j] * sc - m;
+                    c2 = 1.f;
+                    mk = lift<CT>(x.len);
+                }
+#pragma unroll
+                for (int j = 0; j < 8; j++) p[j] = __builtin_amdgcn_exp2f(fmaf(p[j], c2, mk));
 #pragma unroll
                 for (int j = 0; j < 4; j++) pf[j] = pack2<QT>(p[2 * j], p[2 * j + 1]);
                 l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
@@ -893,6 +907,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_paged_prompt(
 #pragma unroll
         for (int j = 0; j < 16; j++) acc[i][j] = 0.f;
     float m = kNone, l = 0.f;
+    bool big = false;   // some row's m is
 
     // Vᵀ operand: dims 32 dt + n, key slots (h, j) = keys 32 u + 16 s + 8 (j / 4) + 4 h + j % 4
     auto read_v = [&](int buf, int u, int s, int dt) {
@@ -1009,17 +1024,26 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_paged_prompt(
                 const float mn = fmaxf(m, mx), al = __builtin_amdgcn_exp2f(m - mn);
                 m = mn;
                 l *= al;
+                big = __any(is_big(m));
 #pragma unroll
                 for (int i = 0; i < DT; i++) acc[i] *= al;
             }
-            const float mk = lift<CT>(x.len) - m;
+            float c2 = sc, mk = lift<CT>(x.len) - m;
+            if (__builtin_expect(big, 0) && is_big(m)) {
+#pragma unroll
+                for (int u = 0; u < 2; u++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) sv[u][i] = sv[u][i] * sc - m;
+                c2 = 1.f;
+                mk = lift<CT>(x.len);
+            }
 #pragma unroll
             for (int u = 0; u < 2; u++) {
                 float ls = 0.f;
 #pragma unroll
                 for (int i = 0; i < 16; i += 2) {
-                    const float e0 = __builtin_amdgcn_exp2f(fmaf(sv[u][i], sc, mk));
-                    const float e1 = __builtin_amdgcn_exp2f(fmaf(sv[u][i + 1], sc, mk));
+                    const float e0 = __builtin_amdgcn_exp2f(fmaf(sv[u][i], c2, mk));
+                    const float e1 = __builtin_amdgcn_exp2f(fmaf(sv[u][i + 1], c2, mk));
                     ls += e0 + e1;
                     pf[u][i / 8][(i % 8) / 2] = pack2<QT>(e0, e1);
                 }
