@@ -443,7 +443,7 @@ typedef struct {
     int32_t q_type;        /* QASR_T_F16 or QASR_T_BF16; the cache's own type where that is a 16-bit one */
     int32_t o_type;        /* q_type or QASR_T_F32 */
     int32_t causal, window;
-    float scale;
+    float scale;           /* finite, times log2 e too */
     int32_t max_q, max_kv; /* the most rows / keys that a sequence is expected to have: they choose how the work is split
                               (more are computed all the same, more slowly) */
 } qasr_paged_attn;

@@ -96,7 +96,7 @@ AttnArgs attn_of(const KvPages& c, const qasr_paged_attn* a) {
                QASR_E_INVALID, "paged_attention: q must be f16 or bf16, the cache's own type where that has 16 bits");
     QASR_CHECK(a->o_type == a->q_type || a->o_type == QASR_T_F32, QASR_E_INVALID,
                "paged_attention: o must be of q's type or f32");
-    QASR_CHECK(isfinite(a->scale), QASR_E_INVALID, "paged_attention: scale must be finite");
+    QASR_CHECK(isfinite(a->scale * (float)M_LOG2E), QASR_E_INVALID, "paged_attention: scale must be finite, times log2 e too");
     QASR_CHECK(a->window >= 0 && a->max_q >= 0 && a->max_kv >= 0, QASR_E_INVALID, "paged_attention: negative size");
     // no position lies further than 2^30 from another
     return AttnArgs{a->n_heads, a->q_type, a->o_type, a->causal != 0, a->window < 1 << 30 ? a->window : 1 << 30, a->max_q, a->max_kv, a->scale};

@@ -114,6 +114,19 @@ def test_attention_refused(kw):
                                         None))
 
 
+@pytest.mark.parametrize("scale,ok", [(2.3e38, True), (-2.3e38, True), (2.4e38, False), (-3.4e38, False),
+                                      (float("nan"), False)])
+def test_attention_scale_fits_with_log2e(scale, ok):
+    """scores are taken to base 2: a scale that is no longer finite then is refused, not answered with NaN"""
+    lib, n = _lib.load(), C.c_size_t()
+    rc = lib.qasr_paged_attention_workspace(C.byref(cache()), C.byref(attn(scale=scale)), C.byref(n))
+    assert (rc == 0) == ok
+    if not ok:
+        refused(rc)
+        refused(lib.qasr_op_paged_attention(C.byref(cache()), C.byref(attn(scale=scale)), A, 512, A, A, 3, A, 512, A,
+                                            1 << 40, None))
+
+
 def test_attention_arguments_refused():
     lib, n = _lib.load(), C.c_size_t()
     refused(lib.qasr_paged_attention_workspace(C.byref(cache()), C.byref(attn()), None))
