@@ -219,6 +219,8 @@ QASR_API int qasr_op_paged_attention(const qasr_kv_cache* c, const qasr_paged_at
         if (rows == 0 || p.n_seq == 0) return;
         QASR_CHECK(q && o && q_start && kv_len && aligned(q_start, 4) && aligned(kv_len, 4), QASR_E_INVALID,
                    "paged_attention: NULL argument");
+        QASR_CHECK(q != o || (at.q_type == at.o_type && ldq == ldo), QASR_E_INVALID,
+                   "paged_attention: in place needs one type and stride");
         const size_t need = paged_attention_ws(p, at);
         QASR_CHECK(need == 0 || (ws && aligned(ws, 128) && ws_bytes >= need), QASR_E_CAPACITY,
                    "paged_attention: the workspace is smaller than qasr_paged_attention_workspace says, or misaligned");

@@ -11,6 +11,8 @@
 // Few rows (k_paged_attn): bound by memory.  16 / 8 heads of 128, f16: one sequence of 32,768 keys 32 us (134 MB, 4.1 TB/s),
 // 64 of 17 .. 8,200 92 us (396 MB, 4.3 TB/s); over 4-bit pages 32 of 501 .. 32,768 76 us (322 MB, 4.2 TB/s; a copy of
 // 2 GiB runs at 4.8).  A token of one sequence of 403 keys: 9 us, all of it round trips.
+// o may be q: an item's rows of q are read by its own workgroups alone, into registers, and its o is written when all of
+// them have done with them (no __restrict__ on either: the compiler must not load q again behind a store).
 // Many rows (k_paged_prompt): bound by the matrix unit and the softmax in turn.  8,192 × 8,192: 600 us, 920 TFLOP/s, causal
 // 870; over 4-bit pages 945 and 865 (a large f16 product of the library: 1,180).
 #include "lds_dma.h"
@@ -326,9 +328,9 @@ __device__ __forceinline__ void store_out(void* o, int o_type, int64_t at, f32x4
 // (m, l, Oᵀ) in the scratch, and the last of the item's workgroups to arrive adds them up in their order (the result does
 // not depend on who is last).  Slot 0 of a workgroup: the item began in an earlier one; slot 1: it goes on in a later one.
 template <int HD, int CT, int QT>
-__global__ __launch_bounds__(256, wgs_per_cu(HD, CT)) void k_paged_attn(KvPages c, AttnArgs a, const void* __restrict__ q, int64_t ldq,
+__global__ __launch_bounds__(256, wgs_per_cu(HD, CT)) void k_paged_attn(KvPages c, AttnArgs a, const void* q, int64_t ldq,
                                                        const int* __restrict__ q_start, const int* __restrict__ kv_len,
-                                                       int rows, void* __restrict__ o, int64_t ldo, float* part,
+                                                       int rows, void* o, int64_t ldo, float* part,
                                                        unsigned* cnt, int q_vec, int o_vec) {
     constexpr int ND = HD / 16, KK = HD / 32, LANES = 64;
     constexpr int kSlot = 16 * HD + 32;   // floats of a slot: Oᵀ as [wave][lane >> 4][row][ND], then m and l of 16 rows
@@ -753,8 +755,8 @@ __device__ __forceinline__ int v_swz(int row) { return HD == 64 ? (row & 2) << 1
 
 template <int HD, int CT, int QT>
 __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_paged_prompt(
-    KvPages c, AttnArgs a, const void* __restrict__ q, int64_t ldq, const int* __restrict__ q_start,
-    const int* __restrict__ kv_len, int rows, void* __restrict__ o, int64_t ldo, float* part, unsigned* cnt, int splits,
+    KvPages c, AttnArgs a, const void* q, int64_t ldq, const int* __restrict__ q_start,
+    const int* __restrict__ kv_len, int rows, void* o, int64_t ldo, float* part, unsigned* cnt, int splits,
     int fill, int q_vec, int o_vec) {
     constexpr int KK = HD / 16, DT = HD / 32, CPR = HD / 8, ROW = HD * 2;
     constexpr bool kAhead = CT == T_MXFP4 || HD == 256;

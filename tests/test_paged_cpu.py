@@ -142,6 +142,12 @@ def test_attention_arguments_refused():
                                            0, None))
 
 
+@pytest.mark.parametrize("kw,ld", [(dict(o_type=_lib.T_F32), (512, 512)), (dict(), (512, 520))])
+def test_attention_in_place_of_another_type_or_stride(kw, ld):
+    refused(_lib.load().qasr_op_paged_attention(C.byref(cache()), C.byref(attn(**kw)), A, ld[0], A, A, 3, A, ld[1], A, 1 << 40,
+                                                None))
+
+
 def test_fp4_plain_form():
     """borders between codes go to the even code, the exponent is the smallest that holds the block's maximum"""
     x = np.zeros((1, 32), np.float32)

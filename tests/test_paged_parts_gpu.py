@@ -115,3 +115,20 @@ def test_parts_with_holes_and_odd_rows(torch_dev, kv, qt, hd, max_q):
     attend(c, q, qs, kl, 2, True, 0, 0.02, ot="f32", o=o, max_q=max_q)
     check(c, q, o, qs, kl, 2, True, 0, 0.02, qt, "f32", rows=np.arange(75) != 69, values=clean)
     assert not np.isfinite(num(o)[69, : 2 * hd]).any()
+
+
+@pytest.mark.parametrize("kv,qt", LAYOUTS)
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("max_q", [1, 1000])
+def test_output_in_place_of_q(torch_dev, kv, qt, hd, max_q):
+    """o written over q gives what a second buffer gets, bit for bit: whole items and shared ones, rows without a key, and rows
+    of no sequence as they were"""
+    rng = np.random.default_rng(hd)
+    lens, nq = [3100, 0, 5003, 40, 1], [70, 2, 9, 60, 1]
+    c, q, qs, kl = marked(rng, kv, qt, 32, 2, 3, hd, lens, nq)
+    q = c.torch.cat((q, q[:3]))
+    want = attend(c, q, qs, kl, 6, True, 0, 0.05, max_q=max_q)
+    for _ in range(3):
+        x = q.clone()
+        attend(c, x, qs, kl, 6, True, 0, 0.05, o=x, max_q=max_q)
+        assert c.torch.equal(x[:-3], want[:-3]) and c.torch.equal(x[-3:], q[-3:])
