@@ -132,3 +132,27 @@ def test_output_in_place_of_q(torch_dev, kv, qt, hd, max_q):
         x = q.clone()
         attend(c, x, qs, kl, 6, True, 0, 0.05, o=x, max_q=max_q)
         assert c.torch.equal(x[:-3], want[:-3]) and c.torch.equal(x[-3:], q[-3:])
+
+
+@pytest.mark.parametrize("kv,qt", LAYOUTS)
+@pytest.mark.parametrize("max_q", [1, 1000])
+def test_long_sequences_among_many(torch_dev, kv, qt, max_q):
+    """more sequences than a wave holds at once, long ones (shared out) beside short and empty ones in each stretch of 64"""
+    rng = np.random.default_rng(21)
+    lens, nq = rng.integers(0, 60, 150), rng.integers(0, 3, 150)
+    for s, n in ((3, 2500), (63, 4100), (64, 3000), (100, 5000), (149, 2000)):
+        lens[s], nq[s] = n, 2
+    c, q, qs, kl = marked(rng, kv, qt, 16, 1, 2, 64, lens, nq)
+    o = attend(c, q, qs, kl, 2, True, 0, 0.02, max_q=max_q)
+    got, rows = num(o), np.concatenate([np.arange(qs[s], qs[s + 1]) for s in (3, 63, 64, 100, 149)])
+    # every row against the plain form; the groups' shares of the long ones
+    c2, q2 = c, q[dev(rows)]
+    c2.table_h = c.table_h[[3, 63, 64, 100, 149]]
+    long = c.torch.from_numpy(got[rows])
+    check(c2, q2, long, np.arange(0, 11, 2), kl[[3, 63, 64, 100, 149]], 2, True, 0, 0.02, qt, qt)
+    short = np.setdiff1d(np.arange(len(got)), rows)
+    assert np.isfinite(got[short]).all() and (got[short] <= 1.01).all() and (got[short] >= 0).all()
+    total = got[short].reshape(len(short), 2, 64).sum(-1)      # V has one mark a key: 1 a row, 0 without keys
+    keys = np.repeat(kl, np.diff(qs))[short]
+    sees = keys > np.maximum(np.repeat(np.diff(qs), np.diff(qs))[short] - 1 - (short - np.repeat(qs[:-1], np.diff(qs))[short]), 0)
+    assert (np.abs(total - sees[:, None]) <= 4 * u_of(qt)).all()
