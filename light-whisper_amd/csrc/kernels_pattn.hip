@@ -1192,12 +1192,12 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_paged_prompt(
 // against 25 us, of 8,192 46 against 40; 4 of 2,000 66 against 30; 16 of 2,000 102 against 46), over 4-bit ones up to 16,384
 // keys (256 rows: 64 x 2,000 keys 67 against 108 us, 16 x 8,192 127 against 124, 4 x 32,768 284 against 199)
 enum Rule { kFew, kMid, kMany };
-static Rule rule_of(const KvPages& c, const AttnArgs& a) {
-    const int64_t r = (int64_t)a.max_q * (a.nh / c.nkv);
+static Rule rule_of(int G, const AttnArgs& a) {
+    const int64_t r = (int64_t)a.max_q * G;
     return r <= 64 ? kFew : r <= 256 ? kMid : kMany;
 }
 static bool is_prompt(const KvPages& c, const AttnArgs& a, int64_t row_tiles) {
-    const Rule rule = rule_of(c, a);
+    const Rule rule = rule_of(a.nh / c.nkv, a);
     if (rule != kMid) return rule == kMany;
     const int64_t keys = a.window > 0 ? std::min((int64_t)a.max_kv, (int64_t)a.window + a.max_q) : a.max_kv;
     if (c.type == T_MXFP4) return keys > 16384;
@@ -1207,7 +1207,7 @@ static bool is_prompt(const KvPages& c, const AttnArgs& a, int64_t row_tiles) {
 size_t paged_attention_ws(const KvPages& c, const AttnArgs& a) {
     const size_t few = (size_t)kSplitWgs * 4 + (size_t)kSplitWgs * 2 * (16 * c.hd + 32) * 4;
     const size_t many = (size_t)kSplitWgs * 4 + (size_t)kPromptSlots * kRowBlock * (c.hd + 2) * 4;
-    return rule_of(c, a) == kFew ? few : std::max(few, many);
+    return rule_of(a.nh / c.nkv, a) == kFew ? few : std::max(few, many);
 }
 
 template <int HD, int CT, int QT>
