@@ -6,7 +6,8 @@
 //   Oᵀ = Vᵀ·Pᵀ  (dims × rows; a lane's weights are the second operand as they stand, V is brought to match)
 // One pass over the keys with a running maximum that moves only where some row's rises by more than 2^kSlack: weights are
 // exp2(s − m + lift), sums and Oᵀ in f32.  Roundings: the weights to q's type for the product with V (half a step each; f16
-// reaches 2^-26 of the largest before its steps stop shrinking), the output to its type.  e2m1 · 2^E is exact in either type.
+// reaches 2^-26 of the largest before its steps stop shrinking), and their sum is that of the rounded ones, so that an output
+// lies between the values it is a mean of; the output to its type.  e2m1 · 2^E is exact in either type.
 //
 // Few rows (k_paged_attn): bound by memory.  16 / 8 heads of 128, f16: one sequence of 32,768 keys 32 us (134 MB, 4.1 TB/s),
 // 64 of 17 .. 8,200 92 us (396 MB, 4.3 TB/s); over 4-bit pages 32 of 501 .. 32,768 76 us (322 MB, 4.2 TB/s; a copy of
@@ -76,6 +77,17 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     const f32x2 v = {a, b};
     if constexpr (QT == T_F16) return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2));
     else return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
+}
+// sum + both numbers of a packed pair, in f32
+template <int QT>
+__device__ __forceinline__ float add2(uint32_t pair, float sum) {
+    if constexpr (QT == T_F16) {
+        const f16x2 one = {(_Float16)1.f, (_Float16)1.f};
+        return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, pair), one, sum, false);
+    } else {
+        const bf16x2 one = {(__bf16)1.f, (__bf16)1.f};
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pair), one, sum, false);
+    }
 }
 // byte SEL of w: two e2m1 codes · the power of two `s` → a packed pair of QT, exact
 template <int QT>
@@ -572,7 +584,7 @@ __global__ __launch_bounds__(256, wgs_per_cu(HD, CT)) void k_paged_attn(KvPages 
                 for (int j = 0; j < 8; j++) p[j] = __builtin_amdgcn_exp2f(fmaf(p[j], c2, mk));
 #pragma unroll
                 for (int j = 0; j < 4; j++) pf[j] = pack2<QT>(p[2 * j], p[2 * j + 1]);
-                l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+                l += add2<QT>(pf[3], add2<QT>(pf[2], add2<QT>(pf[1], add2<QT>(pf[0], 0.f))));
                 if (!careful) {
 #pragma unroll
                     for (int b = 0; b < ND / 2; b++) {
@@ -1040,17 +1052,13 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_paged_prompt(
                 mk = lift<CT>(x.len);
             }
 #pragma unroll
-            for (int u = 0; u < 2; u++) {
-                float ls = 0.f;
+            for (int u = 0; u < 2; u++)
 #pragma unroll
                 for (int i = 0; i < 16; i += 2) {
                     const float e0 = __builtin_amdgcn_exp2f(fmaf(sv[u][i], c2, mk));
                     const float e1 = __builtin_amdgcn_exp2f(fmaf(sv[u][i + 1], c2, mk));
-                    ls += e0 + e1;
                     pf[u][i / 8][(i % 8) / 2] = pack2<QT>(e0, e1);
                 }
-                l += ls;
-            }
         }
         if (__builtin_expect(odd != 0, 0)) {
             for (uint64_t todo = active ? odd : 0; todo; todo &= todo - 1) {
@@ -1087,6 +1095,12 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_paged_prompt(
         }
         __builtin_amdgcn_s_setprio(1);
         if (active) {
+            float ls[4] = {};   // the weights' sum goes into the shadow of the products
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+#pragma unroll
+                for (int us = 0; us < 4; us++) ls[us] = add2<QT>(pf[us >> 1][us & 1][j], ls[us]);
+            l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
             if constexpr (kAhead) {
                 u32x4 vf[DT];
 #pragma unroll

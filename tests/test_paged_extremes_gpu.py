@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 import paged_ref as ref
-from test_paged_gpu import LAYOUTS, SUB, U32, Cache, attend, dev, make, num, u_of
+from test_paged_gpu import LAYOUTS, SUB, U32, append, attend, dev, make, num, u_of
 
 pytestmark = pytest.mark.gpu
 
@@ -84,3 +84,53 @@ def test_scores_near_the_largest_f32(torch_dev, size):
     for max_q in (1, 1000):
         o = attend(c, q, qs, kl, 4, True, 0, 1.0, max_q=max_q)
         check(c, q, o, qs, kl, 4, 1.0, "bf16", "bf16")
+
+
+@pytest.mark.parametrize("kv", ["f16", "bf16"])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_the_largest_value_of_the_type(torch_dev, kv, hd):
+    """V at the type's largest value, one sign a dim: any mean of it is that value.  All keys but each sequence's first have
+    the weight (1 + 1.1 u) / 2, which is rounded up by 0.9 of its u: that must not carry the output to infinity."""
+    rng = np.random.default_rng(hd)
+    lens, nq = [1, 3, 700, 90, 6000, 17], [1, 2, 30, 90, 2, 1]
+    c, q, qs, kl = make(rng, kv, 32, 2, 2, hd, lens, nq, kv)
+    top, u = float(c.torch.finfo(q.dtype).max), u_of(kv)
+    sign = dev(rng.choice([-1.0, 1.0], hd).astype(np.float32), kv)
+    c.pools[1].copy_((sign * top).expand_as(c.pools[1]))
+    for p, x in ((c.pools[0], -1.0), (q.view(-1, 4, hd), 1.0)):
+        p.zero_()
+        p[..., 0] = x
+    for s in range(len(lens)):
+        c.pools[0][int(c.table_h[s, 0]), :, 0] = 0
+    scale = float(-np.log((1 + 1.1 * u) / 2))
+    for max_q in (1, 1000):     # either way of splitting the work
+        o = attend(c, q, qs, kl, 4, True, 0, scale, max_q=max_q)
+        # the weights' rounding and the output's half step, all of the value itself
+        got, want = num(o).reshape(-1, 4, hd), num(sign) * top
+        assert (np.abs(got - want) <= top * (2 * u + 64 * U32 + u * 1.01)).all()
+
+
+@pytest.mark.parametrize("kv,qt", LAYOUTS)
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_means_of_one_value(torch_dev, kv, qt, hd):
+    """V the same for every key: its mean is that value whatever the weights are rounded to, for they are divided by the sum of
+    what they were rounded to.  At random scores, and with one key before 20,000 of 2^-27 of its weight, where f16 has no
+    leading one left.  32-bit sums are off by 2^-24 for each of up to keys / 32 steps, twice, and 64 besides."""
+    rng = np.random.default_rng(hd)
+    lens, nq = [1, 700, 90, 20000], [1, 3, 90, 2]
+    c, q, qs, kl = make(rng, kv, 32, 2, 2, hd, lens, nq, qt)
+    seq = np.concatenate([np.full(n, s) for s, n in enumerate(lens)]).astype(np.int32)
+    pos = np.concatenate([np.arange(n) for n in lens]).astype(np.int32)
+    v = dev(np.full((len(seq), 2 * hd), 1.5, np.float32))
+    k = rng.standard_normal((len(seq), 2, hd)).astype(np.float32)
+    for scale in (0.09, float(27 * np.log(2))):
+        if scale > 1:
+            k[:] = 0
+            k[..., 0] = np.where(pos == 0, 0, -1)[:, None]
+            q.zero_()
+            q.view(-1, 4, hd)[..., 0] = 1
+        append(c, dev(k.reshape(len(seq), -1)), v, "f32", seq, pos)
+        for max_q in (1, 1000):     # either way of splitting the work
+            o = num(attend(c, q, qs, kl, 4, True, 0, scale, ot="f32", max_q=max_q))
+            steps = 64 + 2 * np.repeat(kl, nq)[:, None] / 32
+            assert (np.abs(o - 1.5) <= 1.5 * U32 * steps).all()
