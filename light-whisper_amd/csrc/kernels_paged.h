@@ -29,7 +29,7 @@ struct Rows {
     int64_t ld;
 };
 
-// per frequency: what the table kernel multiplies positions with (rot / 2 ≤ kRopeFreqs)
+// what a table's frequencies follow from
 struct RopeFreqs {
     int kind, rot;
     double log2_theta, inv_factor, lo, inv_span, mscale;

@@ -92,7 +92,7 @@ __device__ void head_to_lds(const void* x, int64_t off, int hd, const RopeArgs& 
 // the half layout (each pair in one thread), 8 u and hd/2 + 8 u in the interleaved one, and the two halves of the dims that
 // do not rotate likewise.  The head's hd / 16 threads are neighbours, so a run of lanes reads a run of bytes (a lane's 16
 // dims in one piece: a third slower) and the norm's sum is a few xor-shuffles.  A thread takes up to four heads of its row
-// with one read of the table.  Bound by memory: 8,192 rows of 16 heads, bf16, half of each turned, 69 MB in 18 us (3.8 TB/s;
+// with one read of the table.  Bound by memory: 8,192 rows of 16 heads, bf16, half of each turned, 69 MB in 18 us (3.9 TB/s;
 // a copy of 2 GiB runs at 4.8).
 
 // 8 elements as they were loaded; they are widened only when they are used, so that many loads are in flight
@@ -356,8 +356,8 @@ __device__ __forceinline__ void fp4_put(uint8_t* blk, uint32_t codes, int hd, in
 
 // a thread: 16 dims of K (even waves) or V (odd ones) of one KV head, as k_rope_units; hd is a power of two, so every thread
 // has dims.  f32 rows of 8 heads into bf16 pages: 8,191 rows, 101 MB in 23.5 us (4.3 TB/s).  Into 4-bit pages 39 us for 76 MB:
-// there the 64-bit arithmetic of K (below) takes the registers that would hide its loads (in 32 bits 27 us; 32 bits with
-// 64 only next to a border 36, the rare branch takes the same registers; fewer registers by force spill: 67 and more)
+// there K is in 64 bits (below), and its values pass through scratch memory, 80 bytes a thread (into 16-bit pages and in
+// k_rope_units 48): turn16's two layouts store to different elements of one array behind a run-time branch
 template <int XT, int CT>
 __global__ __launch_bounds__(256) void k_kv_append_units(KvPages c, const void* k, const void* v, int64_t ldk, int64_t ldv,
                                                          const int* __restrict__ seq, const int* __restrict__ pos, int rows,

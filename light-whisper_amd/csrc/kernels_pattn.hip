@@ -9,13 +9,15 @@
 // reaches 2^-26 of the largest before its steps stop shrinking), and their sum is that of the rounded ones, so that an output
 // lies between the values it is a mean of; the output to its type.  e2m1 · 2^E is exact in either type.
 //
-// Few rows (k_paged_attn): bound by memory.  16 / 8 heads of 128, f16: one sequence of 32,768 keys 32 us (134 MB, 4.1 TB/s),
-// 64 of 17 .. 8,200 92 us (396 MB, 4.3 TB/s); over 4-bit pages 32 of 501 .. 32,768 76 us (322 MB, 4.2 TB/s; a copy of
+// Few rows (k_paged_attn): bound by memory.  16 / 8 heads of 128, f16: one sequence of 32,768 keys 33 us (134 MB, 4.1 TB/s),
+// 64 of 17 .. 8,200 93 us (396 MB, 4.2 TB/s); over 4-bit pages 32 of 501 .. 32,768 77 us (322 MB, 4.2 TB/s; a copy of
 // 2 GiB runs at 4.8).  A token of one sequence of 403 keys: 9 us, all of it round trips.
 // o may be q: an item's rows of q are read by its own workgroups alone, into registers, and its o is written when all of
 // them have done with them (no __restrict__ on either: the compiler must not load q again behind a store).
-// Many rows (k_paged_prompt): bound by the matrix unit and the softmax in turn.  8,192 × 8,192: 600 us, 920 TFLOP/s, causal
-// 870; over 4-bit pages 945 and 865 (a large f16 product of the library: 1,180).
+// Many rows (k_paged_prompt): the matrix unit is busy 38 % of the time and the vector unit 38 %, 10 % of it both at once (two
+// prompts of 4,097 and 3,512 rows on 6,891 and 8,192 keys, 431 us; profiles/paged_prompt_counters.txt).  8,192 × 8,192: 620 us,
+// 886 TFLOP/s, causal 836; over 4-bit pages 919 and 839; causal at head_dim 64 680, 256 795 (a large f16 product of the
+// library: 1,180).
 #include "lds_dma.h"
 #include "paged_dev.h"
 #include "wt.h"
@@ -743,11 +745,11 @@ __global__ __launch_bounds__(256, wgs_per_cu(HD, CT)) void k_paged_attn(KvPages 
 //   K  swz = r mod chunks: 8 neighbouring rows' chunks fall in 8 places
 //   V  swz = 4 (r mod 4) (head_dim 64: 4 (r / 2 mod 2)): the 4 rows × 64 bytes of a transposing read's half wave fall in
 //      the 16 places of 256 bytes
-// Work: items (sequence, 128 rows, KV head), the longest first, KV heads side by side (neighbouring workgroups go to
+// Work: items (sequence, 128 rows, KV head), a sequence's longest first, KV heads side by side (neighbouring workgroups go to
 // different XCDs: with 8 heads an XCD's L2 serves one).  Where the items are too few for the chip, `splits` workgroups
 // share one item's keys and the last to arrive joins their parts.
-// (Tried, for two prompts of 4,097 and 3,512 rows on 8,192 and 6,001 keys, 424 us: 8 waves in two groups a phase apart, one
-// multiplying while the other takes its softmax, 550 us; the next tile's scores interleaved with the exponentials, 486 us.)
+// (Tried and slower: 8 waves in two groups a phase apart, one multiplying while the other takes its softmax; the next tile's
+// scores interleaved with the exponentials.)
 constexpr int kRowBlock = 128, kPromptKeys = 64;
 constexpr int kPromptSlots = 1024;   // parts of all items together where items are split
 constexpr int kPromptParts = 32;     // … and of one item
@@ -1201,10 +1203,12 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_paged_prompt(
 
 // Which kernel, by the rows (tokens · heads of a KV head) of a sequence.  The few-row one reads the keys anew for every 16
 // rows, which L2 bears for a while; the prompt one has whole blocks of 128 rows to fill and more to start.  To 64 rows the
-// first (one sequence of 32,768 keys, 64 rows, 16 / 8 heads, f16: 58 against 64 us), past 256 the second; between them, over
-// 16-bit pages the first while its list gives no workgroup more than 5 tiles (f16, 256 rows: one sequence of 2,000 keys 20
-// against 25 us, of 8,192 46 against 40; 4 of 2,000 66 against 30; 16 of 2,000 102 against 46), over 4-bit ones up to 16,384
-// keys (256 rows: 64 x 2,000 keys 67 against 108 us, 16 x 8,192 127 against 124, 4 x 32,768 284 against 199)
+// first (16 / 8 heads of 128, f16, 64 rows of one sequence of 32,768 keys: 53 against 68 us), past 256 the second; between
+// them, over 16-bit pages the first while its list gives no workgroup more than 5 tiles (f16, 256 rows: one sequence of 2,000
+// keys 21 against 25 us, of 8,192 47 against 39; 4 of 2,000 67 against 32; 16 of 2,000 101 against 45), over 4-bit ones up to
+// 16,384 keys (256 rows: 16 x 2,000 keys 44 against 45 us, 16 x 8,192 131 against 126, 4 x 32,768 287 against 203).
+// profiles/paged_attention_choice.txt has both at 342 sizes: the rule is off most at 64 rows of several long sequences over
+// 16-bit pages (4 x 32,768 keys 287 against 117 us)
 enum Rule { kFew, kMid, kMany };
 static Rule rule_of(int G, const AttnArgs& a) {
     const int64_t r = (int64_t)a.max_q * G;
