@@ -433,8 +433,8 @@ QASR_API int qasr_op_kv_gather(const qasr_kv_cache* c, const int32_t* seq, const
    (causal), of these the positions > p - window (window > 0).  o = softmax(scale * q . k) v per head (query head h reads KV head
    h / (n_heads / n_kv_heads)); a row that sees no key gets zeros.  One token per sequence (decode), several (verify
    passes), whole prompts and, without causal, another sequence's states (cross attention) are all this one call.
-   Scores (times log2 e: up to 2.35e38 in size), softmax and sums in 32 bits; the weights are rounded to q's type for the
-   product with V and divided by the sum of the rounded ones.
+   Scores (of at most 2.35e38: they are taken to base 2), softmax and sums in 32 bits; the weights are rounded to q's type
+   for the product with V and divided by the sum of the rounded ones.
    o may be q (same type and stride); otherwise their rows' heads lie apart.
    What lies in a cache outside a sequence's keys is never used, whatever it holds; keys on a page id outside the
    pool are left out.  kv_len is cut to max_pages * page_size (below 0: 0), q_start to [0, rows] and to not falling (an entry
